@@ -92,6 +92,46 @@ NC_API int nc_ext_pipeline_wait_probe(nc_ctx *ctx);
 NC_API int nc_ext_cross_entropy_fwd_noalloc(const float *logits, const int32_t *labels, int64_t rows,
                                             int64_t classes, float *prob, float *loss, int *status, void *stream);
 
+/* ---- tensors on the device -----------------------------------------------------------------------
+ * Address of t's element 0 in device memory (a view's own first element; strides as created), with host
+ * writes pushed and pending values computed. The data is that of the context's stream: a reader or writer on
+ * another stream orders itself after nc_ext_stream (an event, or nc_ext_synchronize) and before the next op.
+ * write != 0 says that the caller will write through the address: host mirrors are dropped. The address
+ * holds until t is released or, for a temporary, until nc_step_end. NULL when t is NULL or holds no data, or
+ * the context has an error. */
+NC_API void *nc_ext_device_data(nc_tensor *t, int write);
+/* nc_backward from any f32 tensor y with dy as the gradient of it (same shape, any strides, same context)
+ * instead of a scalar loss with gradient 1. dy is read, never written or kept. Returns the context status. */
+NC_API int nc_ext_backward_from(nc_tensor *y, nc_tensor *dy);
+
+/* ---- query/key norms with rotary positions -------------------------------------------------------
+ * x [batch, tokens, heads, dim] f32 (any strides; a slice of a fused projection is read in place) holds
+ * query heads, then key heads. Each head's vector is divided by its root mean square (x * (mean x^2 +
+ * eps)^-1/2), multiplied by q_weight (the first q_heads heads) or k_weight (the others), both [dim] f32 or
+ * NULL for none, and rotated by its position: pair i, of dim / 2, is elements (i, dim/2 + i), or (2i, 2i + 1)
+ * with NC_EXT_ROPE_INTERLEAVED. One pass over x; the result is contiguous and has x's shape.
+ *
+ * positions: i32 [tokens, n_axes] or [batch, tokens, n_axes] (time, height, width, ...; any i32 value), or
+ * NULL with one axis: the token's index. The first sections[0] pairs follow axis 0, the next sections[1] axis
+ * 1, and so on; pairs behind the last section are not rotated. Pair i turns by base^(-i / (dim/2)) radians per
+ * step of its axis; with NC_EXT_ROPE_AXIS_FREQ by base^(-j / sections[a]), j counting from the start of its
+ * section, so that every axis has the whole range of frequencies. Angles are formed in 64 bits.
+ * NC_EXT_ROPE_NO_NORM leaves the division out (weights still apply).
+ *
+ * dim is even, 2 to 256; 1 to 3 axes; the sections sum to at most dim / 2. Gradients reach x, q_weight and
+ * k_weight, in an order of summation that is the same every time. */
+enum { NC_EXT_ROPE_INTERLEAVED = 1, NC_EXT_ROPE_AXIS_FREQ = 2, NC_EXT_ROPE_NO_NORM = 4 };
+typedef struct {
+    int q_heads;
+    int n_axes;
+    int sections[3];
+    float base;
+    float eps;
+    int flags;
+} nc_ext_rope_opts;
+NC_API nc_tensor *nc_ext_qk_norm_rope(nc_tensor *x, nc_tensor *q_weight, nc_tensor *k_weight, nc_tensor *positions,
+                                      const nc_ext_rope_opts *opts);
+
 #ifdef __cplusplus
 }
 #endif

@@ -37,6 +37,14 @@ class OptimOpts(Structure):
     _fields_ = [(n, c_float) for n in ("lr", "momentum", "weight_decay", "beta1", "beta2", "eps")]
 
 
+class RopeOpts(Structure):
+    """nc_ext_rope_opts; flags are the ROPE_* values."""
+    _fields_ = [("q_heads", c_int), ("n_axes", c_int), ("sections", c_int * 3), ("base", c_float), ("eps", c_float),
+                ("flags", c_int)]
+
+
+ROPE_INTERLEAVED, ROPE_AXIS_FREQ, ROPE_NO_NORM = 1, 2, 4
+
 P = c_void_p
 I64P = POINTER(c_int64)
 PP = POINTER(c_void_p)
@@ -176,6 +184,9 @@ EXT_SIGNATURES: dict = {
     "nc_ext_timing_reset": (None, [P]),
     "nc_ext_cross_entropy_fwd_noalloc": (c_int, [c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_void_p,
                                                  c_void_p]),
+    "nc_ext_device_data": (c_void_p, [P, c_int]),
+    "nc_ext_backward_from": (c_int, [P, P]),
+    "nc_ext_qk_norm_rope": (P, [P, P, P, P, POINTER(RopeOpts)]),
 }
 
 

@@ -260,8 +260,8 @@ static void plan_release_node(nc_ctx *ctx, nc_node *n, nc_tensor *loss, const bw
     ctx->bwd_tmp_n = 0;
     nc_tensor *o = n->out;
     if (o->grad) { /* a node run inside a fused chain never formed its output gradient */
-        nc__arena_free(ctx, o->grad->data, o->grad->bytes);
-        o->grad = NULL;
+        if (o->grad->flags & NC_TF_OWNS_DATA) nc__arena_free(ctx, o->grad->data, o->grad->bytes);
+        o->grad = NULL; /* (a gradient given by the caller stays the caller's) */
     }
     if (!free_graph || o == loss || !(o->flags & NC_TF_OWNS_DATA) || (o->flags & NC_TF_PERSISTENT)) return;
     if (ptr_set_has(&pl->keep, o->data)) return;
@@ -273,6 +273,36 @@ static void plan_release_node(nc_ctx *ctx, nc_node *n, nc_tensor *loss, const bw
 
 nc_status nc_backward(nc_tensor *loss) { return nc_backward_ex(loss, 0, NULL, 0); }
 
+/* d loss / d loss at the start of a pass: 1 stored into a fresh buffer, or added to one that already
+ * holds a gradient. With dy (the gradient of y given by the caller), a y that some op produced reads the
+ * caller's buffer in place (an alias that owns nothing and is dropped when the pass ends: *lent = 1); a leaf, or a y that holds a gradient already, has dy
+ * copied or added into its own. Returns 0 on failure. */
+static int seed_gradient(nc_ctx *ctx, nc_tensor *y, nc_tensor *dy, int *lent) {
+    *lent = 0;
+    if (dy && y->node && !y->grad && nc_is_contiguous(dy)) {
+        nc__dev(dy);
+        y->grad = nc__tensor_alias(dy, 0);
+        *lent = y->grad != NULL;
+        return *lent;
+    }
+    int acc;
+    if (!dy) {
+        nc_tensor *g = nc__grad_buf_acc(y, &acc);
+        if (!g) return 0;
+        if (acc) nck_add_scalar_inplace(nc__k(ctx), (float *)g->data, 1.0f);
+        else nck_fill_f32(nc__k(ctx), (float *)g->data, 1.0f, nc_numel(y));
+        return 1;
+    }
+    const float *src = nc__contig_f32(dy);
+    nc_tensor *g = src ? nc__grad_buf_set(y, &acc) : NULL;
+    if (!g) return 0;
+    if (acc) nck_axpy(nc__k(ctx), nc_numel(y), 1.0f, src, (float *)g->data);
+    else nck_axpy_set(nc__k(ctx), nc_numel(y), 1.0f, src, (float *)g->data);
+    return 1;
+}
+
+static nc_status backward_pass(nc_tensor *loss, nc_tensor *dy, int flags, nc_tensor *const *keep, int n_keep);
+
 nc_status nc_backward_ex(nc_tensor *loss, int flags, nc_tensor *const *keep, int n_keep) {
     if (!loss) return NC_ERR_ARG;
     nc_ctx *ctx = loss->ctx;
@@ -281,6 +311,32 @@ nc_status nc_backward_ex(nc_tensor *loss, int flags, nc_tensor *const *keep, int
         nc__error(ctx, NC_ERR_SHAPE, "backward: loss must be a single f32 element");
         return ctx->status;
     }
+    return backward_pass(loss, NULL, flags, keep, n_keep);
+}
+
+int nc_ext_backward_from(nc_tensor *y, nc_tensor *dy) {
+    if (!y || !dy) return NC_ERR_ARG;
+    nc_ctx *ctx = y->ctx;
+    if (ctx->status != NC_OK) return ctx->status;
+    if (dy->ctx != ctx) {
+        nc__error(ctx, NC_ERR_ARG, "backward_from: inputs belong to different contexts");
+        return ctx->status;
+    }
+    if (y->dtype != NC_F32 || dy->dtype != NC_F32) {
+        nc__error(ctx, NC_ERR_DTYPE, "backward_from: the tensor and its gradient must be f32");
+        return ctx->status;
+    }
+    if (!nc__same_shape(y, dy)) {
+        char sa[96], sb[96];
+        nc__error(ctx, NC_ERR_SHAPE, "backward_from: gradient %s of a tensor %s",
+                  nc__shape_str(dy->ndim, dy->shape, sa, sizeof sa), nc__shape_str(y->ndim, y->shape, sb, sizeof sb));
+        return ctx->status;
+    }
+    return backward_pass(y, dy, 0, NULL, 0);
+}
+
+static nc_status backward_pass(nc_tensor *loss, nc_tensor *dy, int flags, nc_tensor *const *keep, int n_keep) {
+    nc_ctx *ctx = loss->ctx;
     if (!nc__needs_grad(loss)) {
         nc__error(ctx, NC_ERR_STATE,
                   "backward: loss does not require grad (no parameter reached it, or grad was disabled)");
@@ -310,15 +366,11 @@ nc_status nc_backward_ex(nc_tensor *loss, int flags, nc_tensor *const *keep, int
         }
     }
 
-    /* d loss / d loss = 1: stored into a fresh buffer, added to one that already holds a gradient */
-    int seed_acc;
-    nc_tensor *g = nc__grad_buf_acc(loss, &seed_acc);
-    if (!g) {
+    int lent;
+    if (!seed_gradient(ctx, loss, dy, &lent)) {
         plan_free(&pl);
         return ctx->status;
     }
-    if (seed_acc) nck_add_scalar_inplace(nc__k(ctx), (float *)g->data, 1.0f);
-    else nck_fill_f32(nc__k(ctx), (float *)g->data, 1.0f, nc_numel(loss));
     if (is_grad_leaf(loss) && loss->bw_epoch != pl.epoch) {
         /* a leaf loss: its own gradient is the seed */
         loss->bw_epoch = pl.epoch;
@@ -349,6 +401,7 @@ nc_status nc_backward_ex(nc_tensor *loss, int flags, nc_tensor *const *keep, int
         }
         plan_node_done(n);
     }
+    if (lent) loss->grad = NULL;
     plan_free(&pl);
     nc__cuda_ok(ctx, cudaGetLastError(), "backward");
     return ctx->status;

@@ -126,7 +126,8 @@ struct nc_node {
     X(log_softmax) X(softmax) X(cross_entropy)                                 \
     X(conv2d) X(max_pool2d) X(avg_pool2d) X(dropout) X(batch_norm)             \
     X(linear_int8) X(nll_loss) X(compare) X(cat) X(to_dtype)                   \
-    X(bmm) X(layer_norm) X(masked_fill) X(slice)
+    X(bmm) X(layer_norm) X(masked_fill) X(slice)                                \
+    X(qk_norm_rope)
 
 #define NC_DECLARE_OP(name) extern const nc_op_def nc_op_##name;
 NC_OP_LIST(NC_DECLARE_OP)
@@ -306,6 +307,9 @@ nc_tensor *nc__grad_buf(nc_tensor *t);
  * buffer of a temporary comes back without zero-filling and *acc = 0 (the writer stores); otherwise
  * *acc = 1 (the writer adds). Persistent tensors always get a zero-filled buffer and *acc = 1. */
 nc_tensor *nc__grad_buf_acc(nc_tensor *t, int *acc);
+/* The same for a writer that also sets every element of a persistent tensor's gradient: a new or cleared
+ * buffer of any tensor comes back without zero-filling and *acc = 0. */
+nc_tensor *nc__grad_buf_set(nc_tensor *t, int *acc);
 static inline int nc__needs_grad(const nc_tensor *t) { return (t->flags & NC_TF_REQUIRES_GRAD) != 0; }
 /* A backward whose input gradient is its output gradient element for element in row-major order (a
  * reshape, a contiguous copy) passes the buffer on instead of copying it, when the input has no

@@ -329,6 +329,30 @@ void nck_dw_dw(nck_dev *d, const nck_conv *g, const float *x, const float *gy, f
 void nck_pool_fwd(nck_dev *d, const nck_conv *g, const float *x, float *y, int32_t *arg, int is_max);
 void nck_pool_bwd(nck_dev *d, const nck_conv *g, const float *gy, const int32_t *arg, float *gx, int is_max, int acc);
 
+/* ---- query/key norms with rotary positions ------------------------------------------------------ */
+#define NCK_ROPE_MAX_DIM 256
+/* x [B, T, H, D] by element strides (the last is 1); y, dy and dx are contiguous. Heads below HQ take wq,
+ * the others wk (NULL: no weight). Position of axis a at token (b, t): pos[b * pos_b + t * pos_t + a], or t
+ * when pos is NULL. Pair i is (i, D/2 + i), or (2i, 2i + 1) when interleaved; it turns turns[i] (in whole
+ * turns) per step of axis[i]. */
+typedef struct {
+    const float *x;
+    int64_t sb, st, sh;
+    const float *wq, *wk;
+    const int32_t *pos;
+    int64_t pos_b, pos_t;
+    int64_t B, T;
+    int H, HQ, D, n_axes;
+    float eps;
+    int norm, interleaved;
+    double turns[NCK_ROPE_MAX_DIM / 2];
+    unsigned char axis[NCK_ROPE_MAX_DIM / 2];
+} nck_rope;
+void nck_rope_fwd(nck_dev *d, const nck_rope *q, float *y);
+/* dx, dwq, dwk: NULL when not wanted; each is added to (acc 1) or stored (acc 0) */
+void nck_rope_bwd(nck_dev *d, const nck_rope *q, const float *dy, float *dx, int acc_x, float *dwq, int acc_q,
+                  float *dwk, int acc_k);
+
 /* ---- GEMM -------------------------------------------------------------------------------------- */
 /* C_b = alpha * op(A_b) op(B_b) + beta * C_b for b in [0, batch); row-major; ta/tb as the newch kernel
  * table (ta: A stored K x M). With reduce_batch, C = alpha * sum_b op(A_b) op(B_b) + beta * C. */

@@ -552,6 +552,26 @@ nc_tensor *nc__grad_buf_acc(nc_tensor *t, int *acc) {
     return t->grad;
 }
 
+nc_tensor *nc__grad_buf_set(nc_tensor *t, int *acc) {
+    if (t->grad && (t->flags & NC_TF_GRAD_CLEARED)) {
+        nc__dev_write(t->grad);
+        t->flags &= ~NC_TF_GRAD_CLEARED;
+        *acc = 0;
+        return t->grad;
+    }
+    if (t->grad || !(t->flags & NC_TF_PERSISTENT)) return nc__grad_buf_acc(t, acc);
+    t->grad = nc__tensor_new(t->ctx, NC_F32, t->ndim, t->shape, 1);
+    *acc = 0;
+    return t->grad;
+}
+
+void *nc_ext_device_data(nc_tensor *t, int write) {
+    if (!t || !t->data || t->ctx->status != NC_OK) return NULL;
+    void *p = nc__dev(t);
+    if (write) nc__dev_write(t);
+    return t->ctx->status == NC_OK ? p : NULL;
+}
+
 /* ---- printing --------------------------------------------------------------------------------- */
 
 void nc_print(const nc_tensor *t) {
