@@ -494,27 +494,28 @@ class _Engine:
 
         self.capi, self.L = capi, capi.load_b200()
         self.ctx = self.L.nc_init(ctypes.byref(capi.Config(0, 1, 0, 0)))
-        self.views = {}
         self.check()
 
     def check(self):
         if not self.L.nc_ok(self.ctx):
             raise RuntimeError(self.L.nc_error(self.ctx).decode())
 
-    def view(self, t, write=0):
+    def view(self, t, held=None, write=0):
+        """t as torch sees it. Made once for a program's state; it keeps the state's memory from being given back."""
         p = self.L.nc_ext_device_data(t, write)
         if not p:
             self.check()
             raise RuntimeError("a tensor without device data")
         n, shape = self.L.nc_ndim(t), self.L.nc_shape(t)
         key = (p, tuple(shape[i] for i in range(n)), self.L.nc_get_dtype(t))
-        if key not in self.views:
-            if len(self.views) > 256:
-                self.views.clear()
+        views = held.views if held else {}
+        if key not in views:
             kind = {self.capi.F32: "<f4", self.capi.I32: "<i4"}[key[2]]
-            face = type("Face", (), {"__cuda_array_interface__": dict(shape=key[1], typestr=kind, data=(p, False), version=2)})
-            self.views[key] = torch.as_tensor(face(), device=DEV)
-        return self.views[key]
+            face = _Face()
+            face.memory = held.memory if held else None
+            face.__cuda_array_interface__ = dict(shape=key[1], typestr=kind, data=(p, False), version=2)
+            views[key] = torch.as_tensor(face, device=DEV)
+        return views[key]
 
     def tensor(self, x, grad=False):
         """A tensor of the framework's that outlives the step, with x's values."""
@@ -524,17 +525,21 @@ class _Engine:
         self.L.nc_persistent_end(self.ctx)
         self.check()
         if x.numel():
-            self.view(t, 1).copy_(x)
+            self.view(t, write=1).copy_(x)
         if grad:
             self.L.nc_set_requires_grad(t, 1)
         return t
 
 
-class _Held:
-    """A program's tensors and optimizer, given back when it drops them."""
+class _Face:
+    """Device memory as torch takes it, and whose it is."""
 
-    def __init__(self, case):
-        self.case, self.tensors, self.optim = case, [], None
+
+class _Memory:
+    """A program's tensors and optimizer, given back when neither it nor a result of it is held any more."""
+
+    def __init__(self):
+        self.tensors, self.optim = [], None
 
     def __del__(self):
         L = _engine.L
@@ -542,7 +547,13 @@ class _Held:
             L.nc_optim_free(self.optim)
         for t in self.tensors:
             L.nc_release(t)
-        _engine.views.clear()
+
+
+class _Held:
+    """What a program has in hand."""
+
+    def __init__(self, case):
+        self.case, self.memory, self.views = case, _Memory(), {}
 
 
 def _prepare_own(case, seed):
@@ -552,7 +563,7 @@ def _prepare_own(case, seed):
     e, s = _engine, _Held(case)
     L, capi = e.L, e.capi
     grad = bool(case.get("train"))
-    hold = lambda x, g=False: s.tensors.append(e.tensor(x, g)) or s.tensors[-1]  # noqa: E731
+    hold = lambda x, g=False: s.memory.tensors.append(e.tensor(x, g)) or s.memory.tensors[-1]  # noqa: E731
     if case["op"] == "rope":
         x, wq, wk, pos, dy = _rope_inputs(case, seed)
         s.x, s.wq, s.wk, s.pos = hold(x, grad), hold(wq, grad), hold(wk, grad), hold(pos)
@@ -574,7 +585,7 @@ def _prepare_own(case, seed):
         pick = lambda flat: [flat[a:a + n] for a, n in spans]  # noqa: E731
         s.params = [hold(x.view(shape), True) for x, shape in zip(pick(w), shapes)]
         o = capi.OptimOpts(HYPER["lr"], 0.0, case["decay"], HYPER["beta1"], HYPER["beta2"], HYPER["eps"])
-        s.optim = L.nc_ext_adamw8(e.ctx, capi.ptr_array(s.params), len(s.params), o)
+        s.optim = s.memory.optim = L.nc_ext_adamw8(e.ctx, capi.ptr_array(s.params), len(s.params), o)
         e.check()
         for p, x, shape in zip(s.params, pick(g), shapes):
             dp = e.tensor(x.view(shape))
@@ -587,8 +598,8 @@ def _prepare_own(case, seed):
         L.nc_ext_optim_put_state(s.optim, s.states)
         L.nc_optim_set_step(s.optim, HYPER["start"])
         L.nc_ext_synchronize(e.ctx)
-        both, at = e.view(s.states, 1), 0
-        s.out = {"w": [e.view(p) for p in s.params], "m": [], "v": []}
+        both, at = e.view(s.states, s, 1), 0
+        s.out = {"w": [e.view(p, s) for p in s.params], "m": [], "v": []}
         for (_, n), shape in zip(spans, shapes):
             s.out["m"].append(both[0, at:at + n].view(shape))
             s.out["v"].append(both[1, at:at + n].view(shape))
@@ -604,12 +615,12 @@ def _run_own(s):
     L.nc_step_end(e.ctx)  # the step before is over
     if case["op"] == "rope":
         if not case["train"]:
-            return e.view(L.nc_ext_qk_norm_rope(s.x, s.wq, s.wk, s.pos, ctypes.byref(s.opts)))
+            return e.view(L.nc_ext_qk_norm_rope(s.x, s.wq, s.wk, s.pos, ctypes.byref(s.opts)), s)
         for t in (s.x, s.wq, s.wk):
             L.nc_clear_grad(t)
         y = L.nc_ext_qk_norm_rope(s.x, s.wq, s.wk, s.pos, ctypes.byref(s.opts))
         L.nc_ext_backward_from(y, s.dy)
-        return e.view(y), *(e.view(L.nc_grad(t)) for t in (s.x, s.wq, s.wk))
+        return e.view(y, s), *(e.view(L.nc_grad(t), s) for t in (s.x, s.wq, s.wk))
     if case["op"] == "adamw8":
         L.nc_optim_step(s.optim)
         L.nc_ext_optim_get_state(s.optim, s.states)
@@ -622,6 +633,6 @@ def _run_own(s):
     else:
         loss = L.nc_ext_preference_loss(s.logits, *s.rest, 0.1, case["smoothing"], ctypes.byref(more))
     if not case["train"]:
-        return e.view(loss), e.view(more.value)
+        return e.view(loss, s), e.view(more.value, s)
     L.nc_backward(loss)
-    return e.view(loss), e.view(more.value), e.view(L.nc_grad(s.logits))
+    return e.view(loss, s), e.view(more.value, s), e.view(L.nc_grad(s.logits), s)
