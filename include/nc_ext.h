@@ -132,6 +132,43 @@ typedef struct {
 NC_API nc_tensor *nc_ext_qk_norm_rope(nc_tensor *x, nc_tensor *q_weight, nc_tensor *k_weight, nc_tensor *positions,
                                       const nc_ext_rope_opts *opts);
 
+/* ---- losses on logits for tuning a language model ---------------------------------------------------
+ * Both take f32 logits [rows, vocab] or [batch, tokens, vocab] (any strides with adjacent vocabulary entries:
+ * a slice of tokens is read in place), i32 labels and mask of the leading shape (mask NULL: every row counts,
+ * else rows whose entry is not 0; other integer types are converted), and return a scalar with gradients to
+ * the logits. Rows that the mask leaves out are not read: their logits, labels and other entries may hold
+ * anything, and their gradient is 0. A counted label outside [0, vocab) is an error (found on the device at
+ * the latest: NC_ERR_ARG at the next synchronisation). Logits of -infinity have probability 0. Log
+ * probabilities are summed and compared in 64 bits; sums run in the same order every time.
+ *
+ * Everything but the logits is a constant: while gradients are enabled, an input of the others that requires
+ * grad is refused. */
+
+/* The clipped policy loss with a KL term: with lp the log probability of a row's action, ratio = exp(lp -
+ * old_logp) and away = ref_logp - lp,
+ *   loss = mean over counted rows of  -min(ratio A, clip(ratio, 1 - clip_low, 1 + clip_high) A)
+ *                                     + kl_coef (exp(away) - away - 1)
+ * (0 when no row counts). old_logp, ref_logp and advantages are f32 of the leading shape; ref_logp may be NULL
+ * when kl_coef is 0. *logp (when logp is not NULL) becomes lp of every row as f32, 0 for rows left out,
+ * without gradient. clip_low lies in [0, 1], clip_high is at least 0, kl_coef finite. */
+typedef struct {
+    float clip_low;
+    float clip_high;
+    float kl_coef;
+} nc_ext_policy_opts;
+NC_API nc_tensor *nc_ext_policy_loss(nc_tensor *logits, nc_tensor *actions, nc_tensor *old_logp, nc_tensor *ref_logp,
+                                     nc_tensor *advantages, nc_tensor *mask, const nc_ext_policy_opts *opts,
+                                     nc_tensor **logp);
+
+/* The preference loss of pairs of answers: logits [2 pairs, tokens, vocab], the preferred answers first, in
+ * the order of the others. With s the sum of an answer's counted log probabilities and h = beta ((s - ref) of
+ * the preferred - (s - ref) of the other),
+ *   loss = mean over pairs of  -(1 - label_smoothing) log sigmoid(h) - label_smoothing log sigmoid(-h)
+ * ref_logp: f32 [2 pairs], the reference model's sums, or NULL for 0. *seq_logp (when seq_logp is not NULL)
+ * becomes s as f32 [2 pairs], without gradient. beta is positive, label_smoothing lies in [0, 0.5]. */
+NC_API nc_tensor *nc_ext_preference_loss(nc_tensor *logits, nc_tensor *labels, nc_tensor *ref_logp, nc_tensor *mask,
+                                         float beta, float label_smoothing, nc_tensor **seq_logp);
+
 #ifdef __cplusplus
 }
 #endif

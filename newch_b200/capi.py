@@ -43,6 +43,11 @@ class RopeOpts(Structure):
                 ("flags", c_int)]
 
 
+class PolicyOpts(Structure):
+    """nc_ext_policy_opts."""
+    _fields_ = [("clip_low", c_float), ("clip_high", c_float), ("kl_coef", c_float)]
+
+
 ROPE_INTERLEAVED, ROPE_AXIS_FREQ, ROPE_NO_NORM = 1, 2, 4
 
 P = c_void_p
@@ -187,6 +192,8 @@ EXT_SIGNATURES: dict = {
     "nc_ext_device_data": (c_void_p, [P, c_int]),
     "nc_ext_backward_from": (c_int, [P, P]),
     "nc_ext_qk_norm_rope": (P, [P, P, P, P, POINTER(RopeOpts)]),
+    "nc_ext_policy_loss": (P, [P] * 6 + [POINTER(PolicyOpts), POINTER(c_void_p)]),
+    "nc_ext_preference_loss": (P, [P] * 4 + [c_float, c_float, POINTER(c_void_p)]),
 }
 
 

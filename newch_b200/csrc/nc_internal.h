@@ -127,7 +127,7 @@ struct nc_node {
     X(conv2d) X(max_pool2d) X(avg_pool2d) X(dropout) X(batch_norm)             \
     X(linear_int8) X(nll_loss) X(compare) X(cat) X(to_dtype)                   \
     X(bmm) X(layer_norm) X(masked_fill) X(slice)                                \
-    X(qk_norm_rope)
+    X(qk_norm_rope) X(policy_loss) X(preference_loss)
 
 #define NC_DECLARE_OP(name) extern const nc_op_def nc_op_##name;
 NC_OP_LIST(NC_DECLARE_OP)

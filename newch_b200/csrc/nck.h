@@ -329,6 +329,47 @@ void nck_dw_dw(nck_dev *d, const nck_conv *g, const float *x, const float *gy, f
 void nck_pool_fwd(nck_dev *d, const nck_conv *g, const float *x, float *y, int32_t *arg, int is_max);
 void nck_pool_bwd(nck_dev *d, const nck_conv *g, const float *gy, const int32_t *arg, float *gx, int is_max, int acc);
 
+/* ---- policy and preference losses on logits ------------------------------------------------------- */
+/* N rows of V logits: row r is z + (r / T) * sb + (r % T) * st, its label lab[r], counted when mask (may be
+ * NULL) is not 0. Outputs, each may be NULL: stat[r] = (max, 1 / sum exp(z - max)), lp64 / lp32 the label's log
+ * probability (0 for rows that do not count; their stat is not written). */
+typedef struct {
+    const float *z;
+    int64_t N, V, T, sb, st;
+    const int32_t *lab, *mask;
+    float *stat;
+    double *lp64;
+    float *lp32;
+    int *status;
+} nck_rows;
+/* the clipped policy loss over those rows (adv NULL: log probabilities only): its mean over the counted rows
+ * in *loss, 1 / count in *scale and each row's gradient factor in coef (both may be NULL) */
+typedef struct {
+    const float *old, *ref, *adv;
+    float clip_low, clip_high, kl;
+    float *coef, *scale, *loss;
+} nck_policy;
+void nck_rows_logp(nck_dev *d, const nck_rows *q, const nck_policy *p);
+/* the preference loss of P pairs: sequences i (preferred) and P + i of T rows each, from the rows' lp64;
+ * seq[2P] (may be NULL) the sequences' sums, coef[2P] (may be NULL) their gradient factors, term[P] scratch */
+typedef struct {
+    int64_t P, T;
+    const float *ref;
+    float beta, smoothing;
+    float *seq, *coef, *loss;
+    double *term;
+} nck_pairs;
+void nck_pref_pairs(nck_dev *d, const nck_pairs *p, const double *lp);
+/* dz[N, V] (contiguous; acc 0: stored) = c (one-hot(label) - softmax(z)), c = up[0] * scale[0] *
+ * coef[r / per_coef] for counted rows, 0 for the others (scale may be NULL: 1) */
+typedef struct {
+    const float *up, *scale, *coef;
+    int64_t per_coef;
+    float *dz;
+    int acc;
+} nck_rows_grad;
+void nck_rows_bwd(nck_dev *d, const nck_rows *q, const nck_rows_grad *g);
+
 /* ---- query/key norms with rotary positions ------------------------------------------------------ */
 #define NCK_ROPE_MAX_DIM 256
 /* x [B, T, H, D] by element strides (the last is 1); y, dy and dx are contiguous. Heads below HQ take wq,
