@@ -169,6 +169,23 @@ NC_API nc_tensor *nc_ext_policy_loss(nc_tensor *logits, nc_tensor *actions, nc_t
 NC_API nc_tensor *nc_ext_preference_loss(nc_tensor *logits, nc_tensor *labels, nc_tensor *ref_logp, nc_tensor *mask,
                                          float beta, float label_smoothing, nc_tensor **seq_logp);
 
+/* ---- AdamW with 8-bit moments ------------------------------------------------------------------------
+ * nc_adamw with 16 bytes of memory traffic and 2.03 bytes of state per element instead of 28 and 8: both
+ * moments are kept as one byte an element and an fp32 maximum s per block of 256 elements of a parameter,
+ *   m = sign(c) s (c / 127)^2, c in [-127, 127];   v = s (c / 255)^4, c in [0, 255], 0 for v = 0 only,
+ * each rounded to the nearest code (in sqrt|m| and v^(1/4)) after the step. The step uses the moments before
+ * that rounding, in fp32. Blocks whose largest value is below 2^-94 count as zero; a gradient that is not
+ * finite makes the moments of its block not finite. The handle works with every nc_optim_* call, gradient
+ * accumulation and data parallelism included; nc_optim_state shows the moments as floats, and floats written
+ * through it are encoded again before the next step (v by its absolute value). Defaults as nc_adamw. */
+NC_API nc_optim *nc_ext_adamw8(nc_ctx *ctx, nc_tensor **params, int n, nc_optim_opts opts);
+/* The moments of an optimizer that keeps two (Adam, AdamW, AdamW in 8 bits, RMSprop with momentum: its momentum
+ * and square average) copied to or from a contiguous f32 tensor [2, elements] on the device: row 0 m, row 1 v, the parameters one
+ * after the other. 8-bit moments are decoded and encoded; encoding what was decoded restores them bit for
+ * bit. Together with nc_optim_get_step / set_step a checkpoint without a host copy. Return the context status. */
+NC_API int nc_ext_optim_get_state(nc_optim *o, nc_tensor *values);
+NC_API int nc_ext_optim_put_state(nc_optim *o, nc_tensor *values);
+
 #ifdef __cplusplus
 }
 #endif

@@ -192,6 +192,9 @@ EXT_SIGNATURES: dict = {
     "nc_ext_device_data": (c_void_p, [P, c_int]),
     "nc_ext_backward_from": (c_int, [P, P]),
     "nc_ext_qk_norm_rope": (P, [P, P, P, P, POINTER(RopeOpts)]),
+    "nc_ext_adamw8": (P, [P, PP, c_int, OptimOpts]),
+    "nc_ext_optim_get_state": (c_int, [P, P]),
+    "nc_ext_optim_put_state": (c_int, [P, P]),
     "nc_ext_policy_loss": (P, [P] * 6 + [POINTER(PolicyOpts), POINTER(c_void_p)]),
     "nc_ext_preference_loss": (P, [P] * 4 + [c_float, c_float, POINTER(c_void_p)]),
 }

@@ -83,14 +83,14 @@ __global__ void __launch_bounds__(256) k_optim(nck_opt_hyper h, const nck_param_
 
 }  // namespace
 
-extern "C" int nck_optim_chunks(const nck_param_seg *segs, int nseg, nck_opt_chunk *chunks) {
+extern "C" int nck_optim_chunks(const nck_param_seg *segs, int nseg, int64_t size, nck_opt_chunk *chunks) {
     int k = 0;
     for (int i = 0; i < nseg; i++) {
-        for (int64_t off = 0; off < segs[i].n; off += NCK_OPT_CHUNK) {
+        for (int64_t off = 0; off < segs[i].n; off += size) {
             if (chunks) {
                 int64_t len = segs[i].n - off;
                 chunks[k].seg = i;
-                chunks[k].len = (int32_t)(len < NCK_OPT_CHUNK ? len : NCK_OPT_CHUNK);
+                chunks[k].len = (int32_t)(len < size ? len : size);
                 chunks[k].off = off;
             }
             k++;

@@ -427,7 +427,7 @@ typedef struct {
     float *m, *v;
     int64_t n;
     int32_t param; /* index into the presence bytes */
-    int32_t pad;
+    int32_t blk;   /* 8-bit states: the parameter's first block */
 } nck_param_seg;
 /* one block's work: elements [off, off + len) of segment seg (off a multiple of 4) */
 typedef struct {
@@ -435,20 +435,41 @@ typedef struct {
     int32_t len;
     int64_t off;
 } nck_opt_chunk;
-enum { NCK_OPT_SGD, NCK_OPT_ADAM, NCK_OPT_ADAMW, NCK_OPT_RMSPROP };
+enum { NCK_OPT_SGD, NCK_OPT_ADAM, NCK_OPT_ADAMW, NCK_OPT_RMSPROP, NCK_OPT_ADAMW8 };
 typedef struct {
     int kind;
     float lr, momentum, weight_decay, beta1, beta2, eps, gs, bc1, bc2;
     int eps_inside_sqrt;
 } nck_opt_hyper;
 #define NCK_OPT_CHUNK 1024 /* elements per block: one float4 per thread (a 422k-parameter model: ~400 blocks) */
-/* fills chunks (when not NULL) for the segments; returns how many there are */
-int nck_optim_chunks(const nck_param_seg *segs, int nseg, nck_opt_chunk *chunks);
+/* fills chunks (when not NULL) of `size` elements for the segments; returns how many there are */
+int nck_optim_chunks(const nck_param_seg *segs, int nseg, int64_t size, nck_opt_chunk *chunks);
 /* One launch over device-resident tables: dsegs[nseg], dchunks[nchunk]; total = elements in all
  * segments (for the timer's byte count). present (device, may be NULL): a segment whose
  * present[param] is 0 is left as it is. */
 void nck_optim_step(nck_dev *d, const nck_opt_hyper *h, const nck_param_seg *dsegs, const nck_opt_chunk *dchunks,
                     int nchunk, int64_t total, const unsigned char *present);
+
+/* AdamW with 8-bit moments: blocks of NCK_OPT8_BLOCK elements, a byte an element (cm signed, cv unsigned;
+ * each parameter padded to whole blocks, the padding's codes 0) and the block's largest values (sm, sv).
+ * segs[].blk is a parameter's first block; chunks of NCK_OPT8_CHUNK elements. */
+#define NCK_OPT8_BLOCK 256
+#define NCK_OPT8_CHUNK 2048 /* a warp per block of states, eight of them a thread block */
+typedef struct {
+    int8_t *cm;
+    unsigned char *cv;
+    float *sm, *sv;
+} nck_opt8;
+void nck_adamw8_step(nck_dev *d, const nck_opt_hyper *h, const nck_opt8 *q, const nck_param_seg *dsegs,
+                     const nck_opt_chunk *dchunks, int nchunk, int64_t total, const unsigned char *present);
+/* a parameter's states as fp32 values: element offsets of the dense and of the flat (aligned) layout */
+typedef struct {
+    int64_t dense, flat;
+    int32_t blk, pad;
+} nck_opt8_span;
+/* values of all parameters' m at val and v at val + second, from the codes (put 0) or to them (put 1) */
+void nck_opt8_values(nck_dev *d, const nck_opt8 *q, const nck_opt8_span *dspans, const nck_opt_chunk *dchunks,
+                     int nchunk, int64_t total, float *val, int64_t second, int dense, int put);
 
 /* ---- int8 quantization -------------------------------------------------------------------------- */
 /* rows of act(x) quantized as nck_quantize_rows does (act: a NCK_UN_* kind applied on the fly, -1 none);

@@ -1,5 +1,5 @@
-/* Optimizers: SGD(+momentum), Adam, AdamW, RMSprop with gradient accumulation, one fused launch
- * per step for all parameters.
+/* Optimizers: SGD(+momentum), Adam, AdamW, AdamW with 8-bit moments, RMSprop with gradient accumulation,
+ * one fused launch per step for all parameters.
  *
  * Update rules, defaults, the accumulation gate and the state-slot layout are newch's
  * (engine/src/optim/optim.c: struct :15-27, create :29-67, defaults :81-104, accumulation :106-130,
@@ -16,7 +16,10 @@
  *     all-reduces overlap the rest of the pass; the step reduces what is left, joins, and updates
  *     from the reduced buffer. A parameter with no gradient on any rank (a presence byte per
  *     parameter, maximum over ranks) is skipped as a single-GPU run skips it; one absent on some
- *     ranks only counts as zero there.
+ *     ranks only counts as zero there;
+ *   - nc_ext_adamw8 keeps m and v as a byte an element with an fp32 maximum per 256 (k_optim8.cu); float
+ *     views of its state (nc_optim_state, nc_ext_optim_get_state / put_state) are decoded and encoded on the
+ *     device, and encoding decoded values gives the same codes, so a checkpoint resumes bit for bit.
  */
 #include "nc_internal.h"
 
@@ -24,7 +27,8 @@
 #include <math.h>
 #include <stdlib.h>
 
-enum { OPT_SGD = NCK_OPT_SGD, OPT_ADAM = NCK_OPT_ADAM, OPT_ADAMW = NCK_OPT_ADAMW, OPT_RMSPROP = NCK_OPT_RMSPROP };
+enum { OPT_SGD = NCK_OPT_SGD, OPT_ADAM = NCK_OPT_ADAM, OPT_ADAMW = NCK_OPT_ADAMW, OPT_RMSPROP = NCK_OPT_RMSPROP,
+       OPT_ADAMW8 = NCK_OPT_ADAMW8 };
 
 typedef struct {
     int p0, p1;      /* parameters [p0, p1) */
@@ -56,6 +60,13 @@ struct nc_optim {
     nck_param_seg *segs, *dsegs;
     nck_opt_chunk *chunks, *dchunks;
     int nseg, nchunk, cap_chunk;
+    /* 8-bit moments: codes and block maxima, elements and blocks of all parameters, and the tables of the
+     * value conversions (every parameter, uploaded at first use) */
+    nck_opt8 q8;
+    int64_t numel, blocks;
+    nck_opt8_span *dspans;
+    nck_opt_chunk *dspan_chunks;
+    int nspan_chunk;
     /* data parallel */
     float *gred;             /* device: gradients averaged over ranks */
     grad_bucket *bk;
@@ -95,6 +106,35 @@ static int adopt_grad(nc_optim *opt, int i) {
     return 1;
 }
 
+static int64_t blocks_of(const nc_tensor *p) { return (nc_numel(p) + NCK_OPT8_BLOCK - 1) / NCK_OPT8_BLOCK; }
+
+/* codes and maxima of the 8-bit moments, all zero */
+static int alloc_state8(nc_optim *o) {
+    const size_t codes = (size_t)(o->blocks ? o->blocks : 1) * NCK_OPT8_BLOCK, tops = codes / NCK_OPT8_BLOCK * sizeof(float);
+    cudaStream_t s = (cudaStream_t)o->ctx->dev.stream;
+    if (o->blocks > INT32_MAX) return 0;
+    if (!(o->q8.cm = (int8_t *)nc__persistent_alloc(o->ctx, codes)) ||
+        !(o->q8.cv = (unsigned char *)nc__persistent_alloc(o->ctx, codes)) ||
+        !(o->q8.sm = (float *)nc__persistent_alloc(o->ctx, tops)) || !(o->q8.sv = (float *)nc__persistent_alloc(o->ctx, tops)))
+        return 0;
+    cudaMemsetAsync(o->q8.cm, 0, codes, s);
+    cudaMemsetAsync(o->q8.cv, 0, codes, s);
+    cudaMemsetAsync(o->q8.sm, 0, tops, s);
+    cudaMemsetAsync(o->q8.sv, 0, tops, s);
+    return 1;
+}
+
+static void free_state8(nc_optim *o) {
+    const size_t codes = (size_t)(o->blocks ? o->blocks : 1) * NCK_OPT8_BLOCK, tops = codes / NCK_OPT8_BLOCK * sizeof(float);
+    if (o->q8.cm) nc__persistent_free(o->ctx, o->q8.cm, codes);
+    if (o->q8.cv) nc__persistent_free(o->ctx, o->q8.cv, codes);
+    if (o->q8.sm) nc__persistent_free(o->ctx, o->q8.sm, tops);
+    if (o->q8.sv) nc__persistent_free(o->ctx, o->q8.sv, tops);
+    if (o->dspans) nc__persistent_free(o->ctx, o->dspans, sizeof(nck_opt8_span) * (size_t)(o->n ? o->n : 1));
+    if (o->dspan_chunks)
+        nc__persistent_free(o->ctx, o->dspan_chunks, sizeof(nck_opt_chunk) * (size_t)(o->nspan_chunk ? o->nspan_chunk : 1));
+}
+
 static nc_optim *create(nc_ctx *ctx, int kind, nc_tensor **params, int n, nc_optim_opts o) {
     for (int i = 0; i < n; i++) {
         nc_tensor *p = params[i];
@@ -125,14 +165,17 @@ static nc_optim *create(nc_ctx *ctx, int kind, nc_tensor **params, int n, nc_opt
         opt->off[i] = opt->total;
         /* keep every parameter's slice 16-byte aligned for vector loads */
         opt->total += (nc_numel(params[i]) + 3) & ~(int64_t)3;
+        opt->numel += nc_numel(params[i]);
+        opt->blocks += blocks_of(params[i]);
     }
     size_t bytes = (size_t)(opt->total ? opt->total : 1) * sizeof(float);
     int adam = kind == OPT_ADAM || kind == OPT_ADAMW;
-    int need1 = adam || o.momentum != 0.0f, need2 = adam || kind == OPT_RMSPROP;
+    int need1 = adam || (kind != OPT_ADAMW8 && o.momentum != 0.0f), need2 = adam || kind == OPT_RMSPROP;
     opt->gflat = (float *)nc__persistent_alloc(ctx, bytes);
     if (!opt->gflat) goto fail;
     if (need1 && !(opt->s1 = (float *)nc__persistent_alloc(ctx, bytes))) goto fail;
     if (need2 && !(opt->s2 = (float *)nc__persistent_alloc(ctx, bytes))) goto fail;
+    if (kind == OPT_ADAMW8 && !alloc_state8(opt)) goto fail;
     cudaStream_t s = (cudaStream_t)ctx->dev.stream;
     if (opt->s1) cudaMemsetAsync(opt->s1, 0, bytes, s);
     if (opt->s2) cudaMemsetAsync(opt->s2, 0, bytes, s);
@@ -165,6 +208,7 @@ void nc_optim_free(nc_optim *o) {
     if (o->s1) nc__persistent_free(ctx, o->s1, bytes);
     if (o->s2) nc__persistent_free(ctx, o->s2, bytes);
     if (o->gred) nc__persistent_free(ctx, o->gred, bytes);
+    free_state8(o);
     if (o->dsegs) nc__persistent_free(ctx, o->dsegs, sizeof(nck_param_seg) * (size_t)(o->n ? o->n : 1));
     if (o->dchunks) nc__persistent_free(ctx, o->dchunks, sizeof(nck_opt_chunk) * (size_t)o->cap_chunk);
     if (o->pres_d) nc__persistent_free(ctx, o->pres_d, (size_t)(o->n ? o->n : 1));
@@ -287,6 +331,15 @@ nc_optim *nc_adamw(nc_ctx *ctx, nc_tensor **params, int n, nc_optim_opts opts) {
     return create(ctx, OPT_ADAMW, params, n, adam_defaults(opts));
 }
 
+nc_optim *nc_ext_adamw8(nc_ctx *ctx, nc_tensor **params, int n, nc_optim_opts opts) {
+    if (!ctx || ctx->status != NC_OK) return NULL;
+    if (n < 0 || (n && !params)) {
+        nc__error(ctx, NC_ERR_ARG, "adamw8: no parameters given");
+        return NULL;
+    }
+    return create(ctx, OPT_ADAMW8, params, n, adam_defaults(opts));
+}
+
 nc_optim *nc_rmsprop(nc_ctx *ctx, nc_tensor **params, int n, nc_optim_opts opts, int eps_inside_sqrt) {
     if (opts.beta2 == 0.0f) opts.beta2 = 0.99f;
     if (opts.eps == 0.0f) opts.eps = 1e-8f;
@@ -339,9 +392,59 @@ void nc_optim_set_lr(nc_optim *o, float lr) {
     if (o) o->o.lr = lr;
 }
 
+/* The 8-bit moments' values out of (put 0) or into (put 1) device floats: m's at val, v's at val + second,
+ * a parameter's at its dense or flat offset. Returns 0 on failure. */
+static int values8(nc_optim *o, float *val, int64_t second, int dense, int put) {
+    nc_ctx *ctx = o->ctx;
+    if (!o->dspans) {
+        nck_opt8_span *spans = (nck_opt8_span *)calloc((size_t)(o->n ? o->n : 1), sizeof(nck_opt8_span));
+        nck_param_seg *segs = (nck_param_seg *)calloc((size_t)(o->n ? o->n : 1), sizeof(nck_param_seg));
+        nck_opt_chunk *chunks = NULL;
+        int64_t at = 0, blk = 0;
+        for (int i = 0; spans && segs && i < o->n; i++) {
+            spans[i].dense = at, spans[i].flat = o->off[i], spans[i].blk = (int32_t)blk;
+            segs[i].n = nc_numel(o->params[i]);
+            at += segs[i].n, blk += blocks_of(o->params[i]);
+        }
+        if (spans && segs) {
+            o->nspan_chunk = nck_optim_chunks(segs, o->n, NCK_OPT8_CHUNK, NULL);
+            const size_t room = sizeof(nck_opt_chunk) * (size_t)(o->nspan_chunk ? o->nspan_chunk : 1);
+            chunks = (nck_opt_chunk *)malloc(room);
+            o->dspan_chunks = (nck_opt_chunk *)nc__persistent_alloc(ctx, room);
+            if (chunks && o->dspan_chunks)
+                o->dspans = (nck_opt8_span *)nc__persistent_alloc(ctx, sizeof(nck_opt8_span) * (size_t)(o->n ? o->n : 1));
+            if (o->dspans) {
+                nck_optim_chunks(segs, o->n, NCK_OPT8_CHUNK, chunks);
+                nc__upload(ctx, o->dspans, spans, sizeof(nck_opt8_span) * (size_t)o->n);
+                nc__upload(ctx, o->dspan_chunks, chunks, sizeof(nck_opt_chunk) * (size_t)o->nspan_chunk);
+            } else if (o->dspan_chunks) {
+                nc__persistent_free(ctx, o->dspan_chunks, room);
+                o->dspan_chunks = NULL;
+            }
+        }
+        free(spans);
+        free(segs);
+        free(chunks);
+        if (!o->dspans) {
+            nc__error(ctx, NC_ERR_OOM, "optimizer: out of memory");
+            return 0;
+        }
+    }
+    nck_opt8_values(nc__k(ctx), &o->q8, o->dspans, o->dspan_chunks, o->nspan_chunk, o->numel, val, second, dense, put);
+    return ctx->status == NC_OK;
+}
+
 static void state_upload_if_dirty(nc_optim *o) {
     if (!o->state_host_dirty) return;
     size_t bytes = (size_t)o->total * sizeof(float);
+    if (o->kind == OPT_ADAMW8) {
+        float *tmp = (float *)nc__persistent_alloc(o->ctx, 2 * bytes);
+        if (!tmp) return;
+        nc__upload(o->ctx, tmp, o->h1, bytes);
+        nc__upload(o->ctx, tmp + o->total, o->h2, bytes);
+        values8(o, tmp, o->total, 0, 1);
+        nc__persistent_free(o->ctx, tmp, 2 * bytes);
+    }
     if (o->s1 && o->h1) nc__upload(o->ctx, o->s1, o->h1, bytes);
     if (o->s2 && o->h2) nc__upload(o->ctx, o->s2, o->h2, bytes);
     o->state_host_dirty = 0;
@@ -350,8 +453,23 @@ static void state_upload_if_dirty(nc_optim *o) {
 float *nc_optim_state(nc_optim *o, int param, int slot) {
     if (!o || param < 0 || param >= o->n || slot < 0 || slot > 1) return NULL;
     float *dev = slot == 0 ? o->s1 : o->s2;
-    if (!dev) return NULL;
-    if (!o->state_host_valid) {
+    const int q8 = o->kind == OPT_ADAMW8;
+    if (!dev && !q8) return NULL;
+    if (!o->state_host_valid && q8) {
+        const size_t bytes = (size_t)(o->total ? o->total : 1) * sizeof(float);
+        if (!o->h1 && cudaMallocHost((void **)&o->h1, bytes) != cudaSuccess) return NULL;
+        if (!o->h2 && cudaMallocHost((void **)&o->h2, bytes) != cudaSuccess) return NULL;
+        state_upload_if_dirty(o);
+        float *tmp = (float *)nc__persistent_alloc(o->ctx, 2 * bytes);
+        if (!tmp) return NULL;
+        nc__cuda_ok(o->ctx, cudaMemsetAsync(tmp, 0, 2 * bytes, (cudaStream_t)o->ctx->dev.stream), "memset");
+        values8(o, tmp, o->total, 0, 0);
+        nc__download(o->ctx, o->h1, tmp, (size_t)o->total * sizeof(float));
+        nc__download(o->ctx, o->h2, tmp + o->total, (size_t)o->total * sizeof(float));
+        nc__persistent_free(o->ctx, tmp, 2 * bytes);
+        if (o->ctx->status != NC_OK) return NULL;
+        o->state_host_valid = 1;
+    } else if (!o->state_host_valid) {
         size_t bytes = (size_t)(o->total ? o->total : 1) * sizeof(float);
         if (o->s1 && !o->h1 && cudaMallocHost((void **)&o->h1, bytes) != cudaSuccess) return NULL;
         if (o->s2 && !o->h2 && cudaMallocHost((void **)&o->h2, bytes) != cudaSuccess) return NULL;
@@ -364,6 +482,59 @@ float *nc_optim_state(nc_optim *o, int param, int slot) {
     o->state_host_dirty = 1;
     return (slot == 0 ? o->h1 : o->h2) + o->off[param];
 }
+
+/* One state tensor holds both moments: row 0 m, row 1 v, the parameters one after the other. */
+static int state_tensor_ok(nc_optim *o, const nc_tensor *t, const char *what) {
+    nc_ctx *ctx = o->ctx;
+    if (o->kind != OPT_ADAMW8 && !(o->s1 && o->s2)) {
+        nc__error(ctx, NC_ERR_STATE, "%s: the optimizer does not keep two moments", what);
+        return 0;
+    }
+    if (t->ctx != ctx) {
+        nc__error(ctx, NC_ERR_ARG, "%s: the tensor belongs to another context", what);
+        return 0;
+    }
+    if (t->dtype != NC_F32) {
+        nc__error(ctx, NC_ERR_DTYPE, "%s: the tensor must be f32", what);
+        return 0;
+    }
+    if (t->ndim != 2 || t->shape[0] != 2 || t->shape[1] != o->numel || !nc_is_contiguous(t)) {
+        char st[96];
+        nc__error(ctx, NC_ERR_SHAPE, "%s: expected a contiguous [2, %lld], got %s", what, (long long)o->numel,
+                  nc__shape_str(t->ndim, t->shape, st, sizeof st));
+        return 0;
+    }
+    return 1;
+}
+
+static int move_state(nc_optim *o, nc_tensor *t, int put) {
+    if (!o || !t) return NC_ERR_ARG;
+    nc_ctx *ctx = o->ctx;
+    if (ctx->status != NC_OK || !state_tensor_ok(o, t, put ? "optim_put_state" : "optim_get_state")) return ctx->status;
+    state_upload_if_dirty(o);
+    if (!put) nc__dev_write(t);
+    float *val = (float *)nc__dev(t);
+    if (ctx->status != NC_OK) return ctx->status;
+    if (o->kind == OPT_ADAMW8) {
+        values8(o, val, o->numel, 1, put);
+    } else {
+        int64_t at = 0;
+        for (int i = 0; i < o->n; i++) {
+            const int64_t n = nc_numel(o->params[i]);
+            for (int k = 0; k < 2 && n; k++) {
+                float *flat = (k ? o->s2 : o->s1) + o->off[i], *dense = val + k * o->numel + at;
+                nc__cuda_ok(ctx, cudaMemcpyAsync(put ? flat : dense, put ? dense : flat, (size_t)n * sizeof(float),
+                                                 cudaMemcpyDeviceToDevice, (cudaStream_t)ctx->dev.stream), "optimizer state");
+            }
+            at += n;
+        }
+    }
+    if (put) o->state_host_valid = 0;
+    return ctx->status;
+}
+
+int nc_ext_optim_get_state(nc_optim *o, nc_tensor *values) { return move_state(o, values, 0); }
+int nc_ext_optim_put_state(nc_optim *o, nc_tensor *values) { return move_state(o, values, 1); }
 
 int64_t nc_optim_get_step(const nc_optim *o) { return o ? o->t : 0; }
 
@@ -379,7 +550,7 @@ void nc_optim_set_step(nc_optim *o, int64_t t) {
 
 void nc_optim_set_opts(nc_optim *o, nc_optim_opts opts) {
     if (!o) return;
-    int adam = o->kind == OPT_ADAM || o->kind == OPT_ADAMW;
+    int adam = o->kind == OPT_ADAM || o->kind == OPT_ADAMW || o->kind == OPT_ADAMW8;
     int has_momentum = !adam && o->s1 != NULL;
     if (!adam && has_momentum != (opts.momentum != 0.0f)) {
         nc__error(o->ctx, NC_ERR_ARG, "optimizer: momentum cannot switch between zero and non-zero (%g -> %g)",
@@ -397,7 +568,8 @@ static int upload_tables(nc_optim *o, const nck_param_seg *segs, int nseg) {
     if (!o->dsegs && !(o->dsegs = (nck_param_seg *)nc__persistent_alloc(ctx, sizeof(nck_param_seg) *
                                                                                 (size_t)(o->n ? o->n : 1))))
         return 0;
-    int nchunk = nck_optim_chunks(segs, nseg, NULL);
+    const int64_t size = o->kind == OPT_ADAMW8 ? NCK_OPT8_CHUNK : NCK_OPT_CHUNK;
+    int nchunk = nck_optim_chunks(segs, nseg, size, NULL);
     if (nchunk > o->cap_chunk) {
         if (o->dchunks) nc__persistent_free(ctx, o->dchunks, sizeof(nck_opt_chunk) * (size_t)o->cap_chunk);
         free(o->chunks);
@@ -407,7 +579,7 @@ static int upload_tables(nc_optim *o, const nck_param_seg *segs, int nseg) {
         if (!o->chunks || !o->dchunks) return 0;
         o->cap_chunk = nchunk;
     }
-    nck_optim_chunks(segs, nseg, o->chunks);
+    nck_optim_chunks(segs, nseg, size, o->chunks);
     if (segs != o->segs) memcpy(o->segs, segs, sizeof(nck_param_seg) * (size_t)nseg);
     nc__upload(ctx, o->dsegs, o->segs, sizeof(nck_param_seg) * (size_t)nseg);
     nc__upload(ctx, o->dchunks, o->chunks, sizeof(nck_opt_chunk) * (size_t)nchunk);
@@ -447,7 +619,7 @@ void nc_optim_step(nc_optim *o) {
     h.eps_inside_sqrt = o->eps_inside_sqrt;
     o->t++;
     h.bc1 = 1.0f, h.bc2 = 1.0f;
-    if (o->kind == OPT_ADAM || o->kind == OPT_ADAMW) {
+    if (o->kind == OPT_ADAM || o->kind == OPT_ADAMW || o->kind == OPT_ADAMW8) {
         h.bc1 = 1.0f - powf(c->beta1, (float)o->t);
         h.bc2 = 1.0f - powf(c->beta2, (float)o->t);
     }
@@ -458,10 +630,12 @@ void nc_optim_step(nc_optim *o) {
      * the device by whether any rank had its gradient */
     nck_param_seg *segs = o->segs + o->n; /* scratch half of the array */
     int nseg = 0;
-    int64_t total = 0;
+    int64_t total = 0, blk = 0;
     for (int i = 0; i < o->n; i++) {
         nc_tensor *p = o->params[i];
         nc_tensor *gt = nc_grad(p);
+        const int64_t first = blk;
+        blk += blocks_of(p);
         if (!gt && !dp) continue;
         if (gt) nc__dev(gt);
         nc__dev_write(p);
@@ -473,10 +647,15 @@ void nc_optim_step(nc_optim *o) {
         sg->v = o->s2 ? o->s2 + o->off[i] : NULL;
         sg->n = nc_numel(p);
         sg->param = i;
+        sg->blk = o->kind == OPT_ADAMW8 ? (int32_t)first : 0;
         total += sg->n;
     }
-    if (nseg && upload_tables(o, segs, nseg))
-        nck_optim_step(nc__k(ctx), &h, o->dsegs, o->dchunks, o->nchunk, total, dp ? o->pres_d : NULL);
+    if (nseg && upload_tables(o, segs, nseg)) {
+        if (o->kind == OPT_ADAMW8)
+            nck_adamw8_step(nc__k(ctx), &h, &o->q8, o->dsegs, o->dchunks, o->nchunk, total, dp ? o->pres_d : NULL);
+        else
+            nck_optim_step(nc__k(ctx), &h, o->dsegs, o->dchunks, o->nchunk, total, dp ? o->pres_d : NULL);
+    }
     o->state_host_valid = 0;
 }
 
