@@ -7,294 +7,377 @@
 //
 // Both passes are bound by HBM: x read and y written (8 bytes an element) forward, x and dy read and dx
 // written (12 bytes) backward, about ten operations an element. A row (one head of one token) belongs to a
-// group of 1 to 32 lanes, each owning up to four pairs as two vector loads, so the norm is a few shuffles and
-// the rotation needs no exchange between lanes. A group walks heads of one token, so a lane computes the sines
-// and cosines of its own pairs once a token and keeps them in registers: no table in memory, no barrier. The
-// angle is reduced in 64 bits (position times turns per step, minus its nearest whole number): positions of a
-// million lose no digits, and the reduced turn, at most one half, is exact to 2^-26 in 32 bits.
+// group of LPR lanes (1 to 32), each owning up to four pairs as two vector loads, so the norm is a few
+// shuffles and the rotation needs no exchange between lanes. A warp takes the same run of heads of 32 / LPR
+// tokens, all lanes in step, so a lane forms the sines and cosines of its own pairs once a token and run,
+// multiplies them by the weights once, and keeps them in registers: no table in memory, no barrier. Warps walk
+// a grid of one full wave. A group need not be a power of two of lanes: three heads of 72 or 80 share a
+// warp on nine or ten lanes each, where two on sixteen would leave half the issue slots idle (24 x 1369 x 24 heads
+// of 72: 88 instead of 102 us).
+//
+// Angles are formed in whole numbers: a pair's turns per step are kept as a 64-bit fraction of a turn, a
+// position times it modulo 2^64 is the fraction of the turn reached, exact to 2^-34 turns at any i32 position,
+// and its upper half splits into quarter turns and a remainder of at most 1/8 turn. On that range sine and cosine
+// are polynomials (interpolation in the remainder's square at Chebyshev nodes), off by less than 1.6 * 2^-24.
 #include "k_common.cuh"
 
 using namespace nck;
 
 namespace {
 
-constexpr int kMaxOwn = 4;  // pairs per lane
+// the arithmetic of two pairs
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) { return make_float2(fmaf(a.x, b.x, c.x), fmaf(a.y, b.y, c.y)); }
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) { return make_float2(a.x * b.x, a.y * b.y); }
+__device__ __forceinline__ float2 neg2(float2 a) { return make_float2(-a.x, -a.y); }
+__device__ __forceinline__ float2 both(float f) { return make_float2(f, f); }
 
-__device__ __forceinline__ void load(const float *p, float (&v)[1]) { v[0] = *p; }
-__device__ __forceinline__ void load(const float *p, float (&v)[2]) {
-    const float2 u = *reinterpret_cast<const float2 *>(p);
-    v[0] = u.x, v[1] = u.y;
-}
-__device__ __forceinline__ void load(const float *p, float (&v)[4]) {
-    const float4 u = *reinterpret_cast<const float4 *>(p);
-    v[0] = u.x, v[1] = u.y, v[2] = u.z, v[3] = u.w;
-}
-
-__device__ __forceinline__ void store(float *p, const float (&v)[1]) { *p = v[0]; }
-__device__ __forceinline__ void store(float *p, const float (&v)[2]) {
-    *reinterpret_cast<float2 *>(p) = make_float2(v[0], v[1]);
-}
-__device__ __forceinline__ void store(float *p, const float (&v)[4]) {
-    *reinterpret_cast<float4 *>(p) = make_float4(v[0], v[1], v[2], v[3]);
+template <int VEC>
+__device__ __forceinline__ void load(const float *p, float (&v)[VEC]) {
+    if constexpr (VEC == 1) {
+        v[0] = *p;
+    } else if constexpr (VEC == 2) {
+        const float2 u = *reinterpret_cast<const float2 *>(p);
+        v[0] = u.x, v[1] = u.y;
+    } else {
+        const float4 u = *reinterpret_cast<const float4 *>(p);
+        v[0] = u.x, v[1] = u.y, v[2] = u.z, v[3] = u.w;
+    }
 }
 
-// How the groups share the work: lanes per group, heads per item, items = tokens x chunks of heads.
+template <int VEC>
+__device__ __forceinline__ void store(float *p, const float (&v)[VEC]) {
+    if constexpr (VEC == 1) *p = v[0];
+    else if constexpr (VEC == 2) *reinterpret_cast<float2 *>(p) = make_float2(v[0], v[1]);
+    else *reinterpret_cast<float4 *>(p) = make_float4(v[0], v[1], v[2], v[3]);
+}
+
+// How warps share the work: an item is `run` heads (of one weight) of the 32 / LPR tokens of a tile; the items
+// of the query heads come first.
 struct RopeGrid {
-    int lpr, per_item;
-    int64_t chunks, items;
+    int run, tiles;          // tiles of tokens
+    int64_t items, q_items;
+    FastDiv by_tiles, by_T;
 };
 
-// The pairs of one row that a lane owns, NJ vectors of VEC pairs: the first and second elements of each
-// pair. Pairs behind the row's end read as zero.
-template <int VEC, int NJ>
+constexpr int kOwn = 4, kTwo = kOwn / 2; // pairs per lane, and their register pairs
+
+// Rows that a lane has in flight, two blocks of 256 threads an SM (128 registers a thread). More blocks of fewer
+// rows keep less in flight for the same registers: forward at 4 x 4680 x 24 heads of 128 takes 81 us with 2
+// blocks of 6 rows (70 at the copy rate), 82 with 3 of 2, 84 with 4 of 2; at 24 x 1369 x 24 heads of 72 82, 89 and
+// 88 us (69 at the copy rate). Backward at the first takes 118 us with 2 of 2 (105 at the copy rate), 132 with 3 of 1, 130 with 2 of 3.
+constexpr int kRowsFwd = 6, kRowsBwd = 2;
+
+// The pairs of one row that a lane owns, kOwn / VEC vectors of VEC pairs: the first and the second elements of
+// each pair. Pairs behind the row's end read as zero.
+template <int VEC, int LPR, bool INTER>
 struct Own {
-    float a[NJ * VEC], b[NJ * VEC];
-    template <bool INTER>
-    __device__ __forceinline__ void get(const float *row, int half, int lpr, int l) {
+    float2 a[kTwo], b[kTwo];
+    static constexpr int NJ = kOwn / VEC;
+    __device__ __forceinline__ void get(const float *row, int half, int l) {
+        float x[kOwn], y[kOwn];
 #pragma unroll
         for (int j = 0; j < NJ; j++) {
-            const int p = (j * lpr + l) * VEC;
-            float u[VEC], v[VEC];
-#pragma unroll
-            for (int i = 0; i < VEC; i++) u[i] = v[i] = 0.0f;
+            const int p = (j * LPR + l) * VEC;
+            float u[VEC] = {}, v[VEC] = {};
             if (p < half) {
-                load(row + (INTER ? 2 * p : p), u);
-                load(row + (INTER ? 2 * p + VEC : half + p), v);
+                load<VEC>(row + (INTER ? 2 * p : p), u);
+                load<VEC>(row + (INTER ? 2 * p + VEC : half + p), v);
             }
 #pragma unroll
             for (int i = 0; i < VEC; i++) {
                 if (INTER) { // u, v hold 2 VEC neighbours: pair i is elements 2i and 2i + 1
-                    a[j * VEC + i] = 2 * i < VEC ? u[(2 * i) % VEC] : v[(2 * i) % VEC];
-                    b[j * VEC + i] = 2 * i + 1 < VEC ? u[(2 * i + 1) % VEC] : v[(2 * i + 1) % VEC];
+                    x[j * VEC + i] = 2 * i < VEC ? u[(2 * i) % VEC] : v[(2 * i) % VEC];
+                    y[j * VEC + i] = 2 * i + 1 < VEC ? u[(2 * i + 1) % VEC] : v[(2 * i + 1) % VEC];
                 } else {
-                    a[j * VEC + i] = u[i];
-                    b[j * VEC + i] = v[i];
+                    x[j * VEC + i] = u[i];
+                    y[j * VEC + i] = v[i];
                 }
             }
         }
+#pragma unroll
+        for (int i = 0; i < kTwo; i++) a[i] = make_float2(x[2 * i], x[2 * i + 1]), b[i] = make_float2(y[2 * i], y[2 * i + 1]);
     }
-    template <bool INTER>
-    __device__ __forceinline__ void put(float *row, int half, int lpr, int l) const {
+    __device__ __forceinline__ void put(float *row, int half, int l) const {
+        const float x[kOwn] = {a[0].x, a[0].y, a[1].x, a[1].y}, y[kOwn] = {b[0].x, b[0].y, b[1].x, b[1].y};
 #pragma unroll
         for (int j = 0; j < NJ; j++) {
-            const int p = (j * lpr + l) * VEC;
+            const int p = (j * LPR + l) * VEC;
             if (p >= half) continue;
             float u[VEC], v[VEC];
 #pragma unroll
             for (int i = 0; i < VEC; i++) {
-                if (INTER) {
-                    const int e = i, f = VEC + i; // elements e of u, f of the 2 VEC neighbours
-                    u[i] = e % 2 ? b[j * VEC + e / 2] : a[j * VEC + e / 2];
-                    v[i] = f % 2 ? b[j * VEC + f / 2] : a[j * VEC + f / 2];
-                } else {
-                    u[i] = a[j * VEC + i];
-                    v[i] = b[j * VEC + i];
-                }
+                const int e = i, f = VEC + i; // INTER: elements e and f of the 2 VEC neighbours
+                u[i] = !INTER ? x[j * VEC + i] : e % 2 ? y[j * VEC + e / 2] : x[j * VEC + e / 2];
+                v[i] = !INTER ? y[j * VEC + i] : f % 2 ? y[j * VEC + f / 2] : x[j * VEC + f / 2];
             }
-            store(row + (INTER ? 2 * p : p), u);
-            store(row + (INTER ? 2 * p + VEC : half + p), v);
+            store<VEC>(row + (INTER ? 2 * p : p), u);
+            store<VEC>(row + (INTER ? 2 * p + VEC : half + p), v);
         }
+    }
+    __device__ __forceinline__ void fill(float f) {
+#pragma unroll
+        for (int i = 0; i < kTwo; i++) a[i] = b[i] = both(f);
     }
 };
 
-__device__ __forceinline__ float group_sum(float v, int lpr, unsigned mask) {
-    for (int o = lpr >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(mask, v, o);
-    return v;
-}
-
-// cos and sin of the lane's pairs at one token
-template <int N>
-__device__ __forceinline__ void turn_of(const nck_rope &q, int64_t b, int64_t t, const double (&turns)[N],
-                                        const int (&axis)[N], float (&c)[N], float (&s)[N]) {
-    int at[3] = {0, 0, 0};
-    if (q.pos) {
-        const int32_t *p = q.pos + b * q.pos_b + t * q.pos_t;
-        at[0] = p[0];
-        if (q.n_axes > 1) at[1] = p[1];
-        if (q.n_axes > 2) at[2] = p[2];
+// The sum over a group's lanes, in all of them. Lanes behind the last whole group get some number.
+template <int LPR>
+__device__ __forceinline__ float group_sum(float v, int lane, int l) {
+    if constexpr ((LPR & (LPR - 1)) == 0) {
+#pragma unroll
+        for (int o = LPR >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
+        return v;
     } else {
-        at[0] = (int)t;
-    }
+        constexpr int kTop = LPR > 8 ? 8 : LPR > 4 ? 4 : 2;
 #pragma unroll
-    for (int i = 0; i < N; i++) {
-        const double full = (double)(axis[i] == 0 ? at[0] : axis[i] == 1 ? at[1] : at[2]) * turns[i];
-        sincospif(2.0f * (float)(full - rint(full)), &s[i], &c[i]);
-    }
-}
-
-template <int VEC, int NJ>
-__device__ __forceinline__ void own_turns(const nck_rope &q, int half, int lpr, int l, double (&turns)[NJ * VEC],
-                                          int (&axis)[NJ * VEC]) {
-#pragma unroll
-    for (int j = 0; j < NJ; j++)
-#pragma unroll
-        for (int i = 0; i < VEC; i++) {
-            const int p = (j * lpr + l) * VEC + i;
-            turns[j * VEC + i] = p < half ? q.turns[p] : 0.0;
-            axis[j * VEC + i] = p < half ? q.axis[p] : 0;
+        for (int o = kTop; o > 0; o >>= 1) {
+            const float u = __shfl_down_sync(~0u, v, o);
+            if (l < o && l + o < LPR) v += u;
         }
+        return __shfl_sync(~0u, v, lane - l);
+    }
 }
 
-template <int VEC, int NJ, bool INTER>
-__global__ void __launch_bounds__(256) k_rope_fwd(const __grid_constant__ nck_rope q, RopeGrid g, float *__restrict__ y) {
-    constexpr int N = VEC * NJ, U = 2; // U rows in flight
-    const int lane = threadIdx.x & 31, l = threadIdx.x & (g.lpr - 1), half = q.D >> 1;
-    const unsigned mask = g.lpr == 32 ? 0xffffffffu : ((1u << g.lpr) - 1u) << (lane & ~(g.lpr - 1));
-    const int64_t groups = (int64_t)gridDim.x * (blockDim.x / g.lpr);
+__device__ __forceinline__ float sum2(float2 s) { return s.x + s.y; }
+
+// The pairs' fractions of a turn per step and their axes, in shared memory: registers are better spent on rows in
+// flight, and the parameters' constant bank serves one address at a time.
+struct Turns {
+    uint64_t step[NCK_ROPE_MAX_DIM / 2];
+    int axis[NCK_ROPE_MAX_DIM / 2];
+    __device__ __forceinline__ void fill(const nck_rope &q) {
+        for (int p = threadIdx.x; p < NCK_ROPE_MAX_DIM / 2; p += blockDim.x) step[p] = q.turns[p], axis[p] = q.axis[p];
+        __syncthreads();
+    }
+    // cos and sin of the lane's pairs at token (b, t)
+    template <int VEC, int LPR>
+    __device__ __forceinline__ void at(const nck_rope &q, int64_t b, int64_t t, int l, float2 (&c)[kTwo], float2 (&s)[kTwo]) const {
+        int pos[3] = {(int)t, 0, 0};
+        if (q.pos) {
+            const int32_t *p = q.pos + b * q.pos_b + t * q.pos_t;
+            pos[0] = p[0];
+            if (q.n_axes > 1) pos[1] = p[1];
+            if (q.n_axes > 2) pos[2] = p[2];
+        }
+        float cv[kOwn], sv[kOwn];
+#pragma unroll
+        for (int i = 0; i < kOwn; i++) {
+            const int p = ((i / VEC * LPR + l) * VEC + i % VEC) & (NCK_ROPE_MAX_DIM / 2 - 1); // (behind the row: any)
+            const int a = axis[p];
+            const int64_t at = a == 0 ? pos[0] : a == 1 ? pos[1] : pos[2];
+            const int32_t turn = (int32_t)(((uint64_t)at * step[p]) >> 32);   // of 2^32
+            const uint32_t quarter = ((uint32_t)turn + (1u << 29)) >> 30;
+            const float g = (float)(int32_t)((uint32_t)turn - (quarter << 30)) * 2.3283064365386963e-10f, g2 = g * g;
+            const float sn = g * fmaf(g2, fmaf(g2, fmaf(g2, -75.401611f, 81.592545f), -41.341663f), 6.2831855f);
+            const float cs = fmaf(g2, fmaf(g2, fmaf(g2, -83.591820f, 64.921234f), -19.739153f), 1.0f);
+            const float x = quarter & 1 ? sn : cs, y = quarter & 1 ? cs : sn;
+            cv[i] = (quarter + 1) & 2 ? -x : x;
+            sv[i] = quarter & 2 ? -y : y;
+        }
+#pragma unroll
+        for (int i = 0; i < kTwo; i++) c[i] = make_float2(cv[2 * i], cv[2 * i + 1]), s[i] = make_float2(sv[2 * i], sv[2 * i + 1]);
+    }
+};
+
+// An item's heads [h0, h1), the lane's token (live: it exists; a lane without one reads the last token).
+template <int LPR>
+struct Item {
+    int h0, h1, tok, b, t;
+    bool live;
+    __device__ __forceinline__ Item(const nck_rope &q, const RopeGrid &g, int64_t it, int sub) {
+        constexpr int per = 32 / LPR;
+        const bool query = it < g.q_items;
+        const uint32_t k = (uint32_t)(query ? it : it - g.q_items), chunk = g.by_tiles.div(k);
+        const int first = query ? 0 : q.HQ, end = query ? q.HQ : q.H;
+        h0 = first + (int)chunk * g.run;
+        h1 = min(h0 + g.run, end);
+        const int64_t at = (int64_t)(k - chunk * (uint32_t)g.tiles) * per + sub, tokens = q.B * q.T;
+        live = sub < per && at < tokens;
+        tok = (int)(at < tokens ? at : tokens - 1);
+        b = (int)g.by_T.div((uint32_t)tok);
+        t = tok - b * (int)q.T;
+    }
+};
+
+template <int VEC, int LPR, bool INTER>
+__global__ void __launch_bounds__(256, 2) k_rope_fwd(const __grid_constant__ nck_rope q, const RopeGrid g, float *__restrict__ y) {
+    constexpr int U = VEC == 4 ? kRowsFwd : kRowsFwd / 2; // (more addresses a row: fewer rows without spills)
+    typedef Own<VEC, LPR, INTER> Row;
+    const int lane = threadIdx.x & 31, l = lane % LPR, half = q.D >> 1;
     const float inv_d = 1.0f / (float)q.D;
-    double turns[N];
-    int axis[N];
-    own_turns<VEC, NJ>(q, half, g.lpr, l, turns, axis);
-    for (int64_t it = (int64_t)blockIdx.x * (blockDim.x / g.lpr) + threadIdx.x / g.lpr; it < g.items; it += groups) {
-        const int64_t tok = it / g.chunks, b = tok / q.T, t = tok - b * q.T;
-        const int h0 = (int)(it - tok * g.chunks) * g.per_item, h1 = min(h0 + g.per_item, q.H);
-        const float *x = q.x + b * q.sb + t * q.st;
-        float *out = y + tok * q.H * q.D;
-        float c[N], s[N];
-        turn_of<N>(q, b, t, turns, axis, c, s);
-        for (int h = h0; h < h1; h += U) {
-            Own<VEC, NJ> row[U];
+    __shared__ Turns turns;
+    turns.fill(q);
+    for (int64_t it = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); it < g.items; it += (int64_t)gridDim.x * 8) {
+        const Item<LPR> m(q, g, it, lane / LPR);
+        const float *x = q.x + m.b * q.sb + m.t * q.st + m.h0 * q.sh;
+        float *out = y + ((int64_t)m.tok * q.H + m.h0) * q.D;
+        Row row[U]; // the first rows are on their way while the angles are formed
+#pragma unroll
+        for (int k = 0; k < U; k++)
+            if (m.h0 + k < m.h1) row[k].get(x + k * q.sh, half, l);
+        // y_a = r (x_a ac - x_b bs), y_b = r (x_b bc + x_a as)
+        float2 ac[kTwo], as[kTwo], bc[kTwo], bs[kTwo];
+        turns.template at<VEC, LPR>(q, m.b, m.t, l, ac, as);
+        const float *w = m.h0 < q.HQ ? q.wq : q.wk;
+        Row ws;
+        if (w) ws.get(w, half, l);
+        else ws.fill(1.0f);
+#pragma unroll
+        for (int i = 0; i < kTwo; i++) {
+            bc[i] = mul2(ac[i], ws.b[i]), bs[i] = neg2(mul2(as[i], ws.b[i]));
+            ac[i] = mul2(ac[i], ws.a[i]), as[i] = mul2(as[i], ws.a[i]);
+        }
+        const auto turn = [&](Row &v, float *to) {
+            float r = 1.0f;
+            if (q.norm) {
+                float2 ss = mul2(v.a[0], v.a[0]);
+                ss = fma2(v.b[0], v.b[0], ss);
+#pragma unroll
+                for (int i = 1; i < kTwo; i++) ss = fma2(v.b[i], v.b[i], fma2(v.a[i], v.a[i], ss));
+                r = rsqrtf(fmaf(group_sum<LPR>(sum2(ss), lane, l), inv_d, q.eps));
+            }
+#pragma unroll
+            for (int i = 0; i < kTwo; i++) {
+                const float2 xa = mul2(v.a[i], both(r)), xb = mul2(v.b[i], both(r));
+                v.a[i] = fma2(xa, ac[i], mul2(xb, bs[i]));
+                v.b[i] = fma2(xb, bc[i], mul2(xa, as[i]));
+            }
+            if (m.live) v.put(to, half, l);
+        };
+        for (int h = m.h0;;) {
 #pragma unroll
             for (int k = 0; k < U; k++)
-                if (h + k < h1) row[k].template get<INTER>(x + (h + k) * q.sh, half, g.lpr, l);
+                if (h + k < m.h1) turn(row[k], out + k * q.D);
+            h += U, x += U * q.sh, out += U * q.D;
+            if (h >= m.h1) break;
 #pragma unroll
-            for (int k = 0; k < U; k++) {
-                if (h + k >= h1) break;
-                Own<VEC, NJ> &v = row[k];
-                if (q.norm) {
-                    float ss = 0.0f;
-#pragma unroll
-                    for (int i = 0; i < N; i++) ss = fmaf(v.a[i], v.a[i], fmaf(v.b[i], v.b[i], ss));
-                    const float r = rsqrtf(fmaf(group_sum(ss, g.lpr, mask), inv_d, q.eps));
-#pragma unroll
-                    for (int i = 0; i < N; i++) v.a[i] *= r, v.b[i] *= r;
-                }
-                if (const float *w = h + k < q.HQ ? q.wq : q.wk) {
-                    Own<VEC, NJ> ws;
-                    ws.template get<INTER>(w, half, g.lpr, l);
-#pragma unroll
-                    for (int i = 0; i < N; i++) v.a[i] *= ws.a[i], v.b[i] *= ws.b[i];
-                }
-#pragma unroll
-                for (int i = 0; i < N; i++) {
-                    const float ua = v.a[i], ub = v.b[i];
-                    v.a[i] = fmaf(ua, c[i], -(ub * s[i]));
-                    v.b[i] = fmaf(ub, c[i], ua * s[i]);
-                }
-                v.template put<INTER>(out + (int64_t)(h + k) * q.D, half, g.lpr, l);
-            }
+            for (int k = 0; k < U; k++)
+                if (h + k < m.h1) row[k].get(x + k * q.sh, half, l);
         }
     }
 }
 
 // part (may be NULL): the block's sums of g n over its query rows and over its key rows, [block][2][D]
-template <int VEC, int NJ, bool INTER>
-__global__ void __launch_bounds__(256) k_rope_bwd(const __grid_constant__ nck_rope q, RopeGrid g,
+template <int VEC, int LPR, bool INTER>
+__global__ void __launch_bounds__(256, 2) k_rope_bwd(const __grid_constant__ nck_rope q, const RopeGrid g,
                                                   const float *__restrict__ dy, float *dx, int acc,
                                                   float *__restrict__ part) {
-    constexpr int N = VEC * NJ;
-    __shared__ float red[256 * 2 * kMaxOwn];
-    const int lane = threadIdx.x & 31, l = threadIdx.x & (g.lpr - 1), half = q.D >> 1;
-    const unsigned mask = g.lpr == 32 ? 0xffffffffu : ((1u << g.lpr) - 1u) << (lane & ~(g.lpr - 1));
-    const int per_block = blockDim.x / g.lpr, mine = threadIdx.x / g.lpr;
-    const int64_t groups = (int64_t)gridDim.x * per_block;
+    constexpr int kPer = 32 / LPR, kGroups = 8 * kPer, U = VEC == 1 ? 1 : kRowsBwd;
+    typedef Own<VEC, LPR, INTER> Row;
+    __shared__ float red[kGroups * 2 * LPR * kOwn];
+    const int lane = threadIdx.x & 31, l = lane % LPR, half = q.D >> 1;
     const float inv_d = 1.0f / (float)q.D;
-    double turns[N];
-    int axis[N];
-    own_turns<VEC, NJ>(q, half, g.lpr, l, turns, axis);
-    Own<VEC, NJ> sum[2];
+    __shared__ Turns turns;
+    turns.fill(q);
+    const int64_t step = (int64_t)gridDim.x * 8;
+    int64_t it = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+#pragma unroll 1
+    for (int side = 0; side < 2; side++) { // query heads, then key heads
+        const float *w = side ? q.wk : q.wq;
+        Row ws, sum;
+        if (w) ws.get(w, half, l);
+        else ws.fill(1.0f);
+        sum.fill(0.0f);
+        for (const int64_t end = side ? g.items : g.q_items; it < end; it += step) {
+            const Item<LPR> m(q, g, it, lane / LPR);
+            const float *x = q.x + m.b * q.sb + m.t * q.st + m.h0 * q.sh;
+            const int64_t at = ((int64_t)m.tok * q.H + m.h0) * q.D;
+            const float *from = dy + at;
+            float *to = dx + at;
+            Row x_row[U], dy_row[U]; // the first rows are on their way while the angles are formed
+            const auto fetch = [&](int h) {
 #pragma unroll
-    for (int i = 0; i < N; i++) sum[0].a[i] = sum[0].b[i] = sum[1].a[i] = sum[1].b[i] = 0.0f;
-    for (int64_t it = (int64_t)blockIdx.x * per_block + mine; it < g.items; it += groups) {
-        const int64_t tok = it / g.chunks, b = tok / q.T, t = tok - b * q.T;
-        const int h0 = (int)(it - tok * g.chunks) * g.per_item, h1 = min(h0 + g.per_item, q.H);
-        const float *x = q.x + b * q.sb + t * q.st;
-        float c[N], s[N];
-        turn_of<N>(q, b, t, turns, axis, c, s);
-        for (int h = h0; h < h1; h++) {
-            const int64_t at = (tok * q.H + h) * q.D;
-            Own<VEC, NJ> v, d;
-            v.template get<INTER>(x + h * q.sh, half, g.lpr, l);
-            d.template get<INTER>(dy + at, half, g.lpr, l);
-            float r = 1.0f;
-            if (q.norm) {
-                float ss = 0.0f;
+                for (int k = 0; k < U; k++)
+                    if (h + k < m.h1) x_row[k].get(x + k * q.sh, half, l), dy_row[k].get(from + k * q.D, half, l);
+            };
+            fetch(m.h0);
+            float2 c[kTwo], s[kTwo];
+            turns.template at<VEC, LPR>(q, m.b, m.t, l, c, s);
+            const auto turn_back = [&](Row &v, Row &d, float *to) {
+                float2 ss = both(0.0f), dot = both(0.0f);
 #pragma unroll
-                for (int i = 0; i < N; i++) ss = fmaf(v.a[i], v.a[i], fmaf(v.b[i], v.b[i], ss));
-                r = rsqrtf(fmaf(group_sum(ss, g.lpr, mask), inv_d, q.eps));
-            }
-#pragma unroll
-            for (int i = 0; i < N; i++) {
-                const float ya = d.a[i], yb = d.b[i];
-                d.a[i] = fmaf(ya, c[i], yb * s[i]);
-                d.b[i] = fmaf(yb, c[i], -(ya * s[i]));
-                v.a[i] *= r, v.b[i] *= r; // n
-            }
-            if (part) {
-                const bool query = h < q.HQ;
-#pragma unroll
-                for (int i = 0; i < N; i++) {
-                    const float ga = d.a[i] * v.a[i], gb = d.b[i] * v.b[i];
-                    sum[0].a[i] += query ? ga : 0.0f, sum[0].b[i] += query ? gb : 0.0f;
-                    sum[1].a[i] += query ? 0.0f : ga, sum[1].b[i] += query ? 0.0f : gb;
+                for (int i = 0; i < kTwo; i++) {
+                    const float2 ya = d.a[i], yb = d.b[i];
+                    d.a[i] = fma2(ya, c[i], mul2(yb, s[i]));
+                    d.b[i] = fma2(yb, c[i], neg2(mul2(ya, s[i])));
+                    ss = fma2(v.a[i], v.a[i], fma2(v.b[i], v.b[i], ss));
+                    dot = fma2(mul2(d.a[i], ws.a[i]), v.a[i], fma2(mul2(d.b[i], ws.b[i]), v.b[i], dot));
                 }
-            }
-            if (!dx) continue;
-            if (const float *w = h < q.HQ ? q.wq : q.wk) {
-                Own<VEC, NJ> ws;
-                ws.template get<INTER>(w, half, g.lpr, l);
-#pragma unroll
-                for (int i = 0; i < N; i++) d.a[i] *= ws.a[i], d.b[i] *= ws.b[i];
-            }
-            if (q.norm) {
-                float dot = 0.0f;
-#pragma unroll
-                for (int i = 0; i < N; i++) dot = fmaf(d.a[i], v.a[i], fmaf(d.b[i], v.b[i], dot));
-                const float m = group_sum(dot, g.lpr, mask) * inv_d;
-#pragma unroll
-                for (int i = 0; i < N; i++) {
-                    d.a[i] = r * fmaf(-m, v.a[i], d.a[i]);
-                    d.b[i] = r * fmaf(-m, v.b[i], d.b[i]);
+                float r = 1.0f, k = 0.0f; // dx = r g w + k x, k = -r^3 sum(g w x) / D
+                if (q.norm) {
+                    const float all = group_sum<LPR>(sum2(ss), lane, l), mean = group_sum<LPR>(sum2(dot), lane, l) * inv_d;
+                    r = rsqrtf(fmaf(all, inv_d, q.eps));
+                    k = -(mean * r) * (r * r);
                 }
-            }
-            if (acc) {
-                Own<VEC, NJ> old;
-                old.template get<INTER>(dx + at, half, g.lpr, l);
+                if (!m.live) return;
+                Row o;
 #pragma unroll
-                for (int i = 0; i < N; i++) d.a[i] += old.a[i], d.b[i] += old.b[i];
+                for (int i = 0; i < kTwo; i++) {
+                    const float2 ga = mul2(d.a[i], both(r)), gb = mul2(d.b[i], both(r));
+                    sum.a[i] = fma2(ga, v.a[i], sum.a[i]);
+                    sum.b[i] = fma2(gb, v.b[i], sum.b[i]);
+                    o.a[i] = fma2(ga, ws.a[i], mul2(both(k), v.a[i]));
+                    o.b[i] = fma2(gb, ws.b[i], mul2(both(k), v.b[i]));
+                }
+                if (dx && acc) { // added to what is there
+                    v.get(to, half, l);
+#pragma unroll
+                    for (int i = 0; i < kTwo; i++) {
+                        o.a[i] = fma2(v.a[i], both(1.0f), o.a[i]);
+                        o.b[i] = fma2(v.b[i], both(1.0f), o.b[i]);
+                    }
+                }
+                if (dx) o.put(to, half, l);
+            };
+            for (int h = m.h0;;) {
+#pragma unroll
+                for (int k = 0; k < U; k++)
+                    if (h + k < m.h1) turn_back(x_row[k], dy_row[k], to + k * q.D);
+                h += U, x += U * q.sh, from += U * q.D, to += U * q.D;
+                if (h >= m.h1) break;
+                fetch(h);
             }
-            d.template put<INTER>(dx + at, half, g.lpr, l);
         }
-    }
-    if (!part) return;
-    for (int k = 0; k < 2; k++) {
+        if (!part) continue;
         __syncthreads();
-        sum[k].template put<INTER>(red + mine * q.D, half, g.lpr, l);
+        if (lane < kPer * LPR) sum.put(red + ((threadIdx.x >> 5) * kPer + lane / LPR) * q.D, half, l);
         __syncthreads();
         for (int d = threadIdx.x; d < q.D; d += blockDim.x) {
             float t = 0.0f;
-            for (int j = 0; j < per_block; j++) t += red[j * q.D + d];
-            part[((int64_t)blockIdx.x * 2 + k) * q.D + d] = t;
+            for (int j = 0; j < kGroups; j++) t += red[j * q.D + d];
+            part[((int64_t)blockIdx.x * 2 + side) * q.D + d] = t;
         }
     }
 }
 
-// dw (+)= the blocks' partial sums, in block order; 32 columns a block, 8 slices of the blocks each
-__global__ void __launch_bounds__(256) k_rope_dw(const float *__restrict__ part, int blocks, int D, float *dwq, int acc_q,
-                                                 float *dwk, int acc_k) {
-    __shared__ double red[8][32];
-    const int col = blockIdx.x * 32 + (threadIdx.x & 31), sl = threadIdx.x >> 5;
+// dw (+)= the blocks' partial sums in a fixed order; 32 columns a block, 32 slices of the blocks each
+__global__ void __launch_bounds__(1024) k_rope_dw(const float *__restrict__ part, int blocks, int D, float *dwq, int acc_q,
+                                                  float *dwk, int acc_k) {
+    __shared__ double red[32][33];
+    cudaGridDependencySynchronize(); // launched early: the sums are written when the kernel before has ended
+    const int lane = threadIdx.x & 31, sl = threadIdx.x >> 5, col = blockIdx.x * 32 + lane;
     double t = 0.0;
-    if (col < 2 * D)
-        for (int b = sl; b < blocks; b += 8) t += (double)part[(int64_t)b * 2 * D + col];
-    red[sl][threadIdx.x & 31] = t;
+    if (col < 2 * D) {
+        constexpr int U = 8; // loads in flight
+        for (int b = sl; b < blocks; b += 32 * U) {
+            float v[U];
+#pragma unroll
+            for (int u = 0; u < U; u++) v[u] = b + 32 * u < blocks ? part[(int64_t)(b + 32 * u) * 2 * D + col] : 0.0f;
+#pragma unroll
+            for (int u = 0; u < U; u++) t += (double)v[u];
+        }
+    }
+    red[sl][lane] = t;
     __syncthreads();
-    if (sl || col >= 2 * D) return;
-    for (int j = 1; j < 8; j++) t += red[j][threadIdx.x];
-    float *dw = col < D ? dwq : dwk;
-    if (!dw) return;
-    float *to = dw + (col < D ? col : col - D);
-    const bool acc = col < D ? acc_q : acc_k;
+    // warp sl sums column sl of the block
+    t = red[lane][sl];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(~0u, t, o);
+    const int c = blockIdx.x * 32 + sl;
+    float *dw = c < D ? dwq : dwk;
+    if (lane || c >= 2 * D || !dw) return;
+    float *to = dw + (c < D ? c : c - D);
+    const bool acc = c < D ? acc_q : acc_k;
     *to = acc ? *to + (float)t : (float)t;
 }
 
@@ -311,41 +394,59 @@ int vector_of(const nck_rope *q, const void *p1, const void *p2) {
     return 1;
 }
 
-// Groups of the smallest power of two lanes that holds a row, whole tokens per group when there are enough
-// tokens to fill the GPU, fewer heads per group (each repeats the token's angles) when there are not.
-RopeGrid split_of(const nck_dev *d, const nck_rope *q, int vec) {
+// A run is all heads of a weight when there are tokens enough for several waves of warps, fewer (down to one)
+// when there are not: a shorter run forms the angles more often, a longer one leaves SMs without work.
+RopeGrid split_of(const nck_dev *d, const nck_rope *q, int lpr) {
     RopeGrid g;
-    const int vecs = (q->D / 2 + vec - 1) / vec;
-    g.lpr = 1;
-    while (g.lpr < vecs && g.lpr < 32) g.lpr <<= 1;
-    const int64_t tokens = q->B * q->T, room = (int64_t)d->sm_count * 2048 / g.lpr;
-    int64_t per = tokens * q->H / room;
-    if (per < 1) per = 1;
-    if (per > q->H) per = q->H;
-    g.per_item = (int)per;
-    g.chunks = (q->H + per - 1) / per;
-    g.items = tokens * g.chunks;
+    const int64_t tokens = q->B * q->T, per = 32 / lpr, tiles = (tokens + per - 1) / per;
+    const int64_t want = (int64_t)d->sm_count * 32;
+    int64_t run = tiles * q->H / want;
+    run = run < 1 ? 1 : run > q->H ? q->H : run;
+    const int64_t kh = q->H - q->HQ;
+    g.run = (int)run;
+    g.tiles = (int)tiles;
+    g.q_items = (q->HQ + run - 1) / run * tiles;
+    g.items = g.q_items + (kh + run - 1) / run * tiles;
+    g.by_tiles = make_fastdiv((uint32_t)tiles);
+    g.by_T = make_fastdiv((uint32_t)q->T);
     return g;
 }
 
-template <int VEC, int NJ>
-void launch_fwd(nck_dev *d, const nck_rope *q, const RopeGrid &g, float *y) {
-    const int64_t blocks = (g.items * g.lpr + 255) / 256;
-    const int grid = (int)(blocks < ((int64_t)1 << 30) ? blocks : (int64_t)1 << 30);
-    if (q->interleaved) k_rope_fwd<VEC, NJ, true><<<grid, 256, 0, NCK_STREAM(d)>>>(*q, g, y);
-    else k_rope_fwd<VEC, NJ, false><<<grid, 256, 0, NCK_STREAM(d)>>>(*q, g, y);
-    NCK_LAUNCHED(d, 1);
-}
-
-template <int VEC, int NJ, bool INTER>
-int launch_bwd(nck_dev *d, const nck_rope *q, const RopeGrid &g, const float *dy, float *dx, int acc, float *part) {
-    static int room = 0;
-    if (!room) room = resident_blocks(d, k_rope_bwd<VEC, NJ, INTER>, 256);
-    const int64_t blocks = (g.items * g.lpr + 255) / 256;
-    const int grid = (int)(blocks < room ? blocks : room);
-    k_rope_bwd<VEC, NJ, INTER><<<grid, 256, 0, NCK_STREAM(d)>>>(*q, g, dy, dx, acc, part);
+template <int VEC, int LPR, bool INTER>
+int launch(nck_dev *d, const nck_rope *q, float *y, const float *dy, float *dx, int acc, float *part) {
+    static int room_fwd = 0, room_bwd = 0;
+    if (!room_fwd) {
+        room_bwd = resident_blocks(d, k_rope_bwd<VEC, LPR, INTER>, 256);
+        room_fwd = resident_blocks(d, k_rope_fwd<VEC, LPR, INTER>, 256);
+    }
+    const RopeGrid g = split_of(d, q, LPR);
+    const int64_t blocks = (g.items + 7) / 8;
+    const int room = y ? room_fwd : room_bwd, grid = (int)(blocks < room ? blocks : room);
+    if (y) k_rope_fwd<VEC, LPR, INTER><<<grid, 256, 0, NCK_STREAM(d)>>>(*q, g, y);
+    else k_rope_bwd<VEC, LPR, INTER><<<grid, 256, 0, NCK_STREAM(d)>>>(*q, g, dy, dx, acc, part);
     NCK_LAUNCHED(d, 1);
     return grid;
+}
+
+// Vectors of four pairs on as many lanes as a row has vectors, up to the number that lets as many rows share a
+// warp; rows that only narrower vectors fit take a whole warp each.
+template <bool INTER>
+int dispatch(nck_dev *d, const nck_rope *q, float *y, const float *dy, float *dx, int acc, float *part) {
+    const int vec = y ? vector_of(q, y, nullptr) : vector_of(q, dy, dx);
+    if (vec == 1) return launch<1, 32, INTER>(d, q, y, dy, dx, acc, part);
+    if (vec == 2) return launch<2, 32, INTER>(d, q, y, dy, dx, acc, part);
+    switch (32 / (q->D / 8)) { // rows to a warp
+    case 32: return launch<4, 1, INTER>(d, q, y, dy, dx, acc, part);
+    case 16: return launch<4, 2, INTER>(d, q, y, dy, dx, acc, part);
+    case 10: return launch<4, 3, INTER>(d, q, y, dy, dx, acc, part);
+    case 8: return launch<4, 4, INTER>(d, q, y, dy, dx, acc, part);
+    case 6: return launch<4, 5, INTER>(d, q, y, dy, dx, acc, part);
+    case 5: return launch<4, 6, INTER>(d, q, y, dy, dx, acc, part);
+    case 4: return launch<4, 8, INTER>(d, q, y, dy, dx, acc, part);
+    case 3: return launch<4, 10, INTER>(d, q, y, dy, dx, acc, part);
+    case 2: return launch<4, 16, INTER>(d, q, y, dy, dx, acc, part);
+    default: return launch<4, 32, INTER>(d, q, y, dy, dx, acc, part);
+    }
 }
 
 }  // namespace
@@ -354,11 +455,8 @@ extern "C" void nck_rope_fwd(nck_dev *d, const nck_rope *q, float *y) {
     const double n = (double)q->B * q->T * q->H * q->D;
     if (n == 0) return;
     Scope sc(d, "qk_norm_rope", 10.0 * n, 8.0 * n);
-    const int vec = vector_of(q, y, nullptr);
-    const RopeGrid g = split_of(d, q, vec);
-    if (vec == 4) launch_fwd<4, 1>(d, q, g, y);
-    else if (vec == 2) launch_fwd<2, 2>(d, q, g, y);
-    else launch_fwd<1, 4>(d, q, g, y);
+    if (q->interleaved) dispatch<true>(d, q, y, nullptr, nullptr, 0, nullptr);
+    else dispatch<false>(d, q, y, nullptr, nullptr, 0, nullptr);
 }
 
 extern "C" void nck_rope_bwd(nck_dev *d, const nck_rope *q, const float *dy, float *dx, int acc_x, float *dwq, int acc_q,
@@ -367,20 +465,16 @@ extern "C" void nck_rope_bwd(nck_dev *d, const nck_rope *q, const float *dy, flo
     Scope sc(d, "qk_norm_rope_bwd", 20.0 * n, 12.0 * n);
     float *part = dwq || dwk ? (float *)d->scratch : nullptr;
     int grid = 0;
-    if (n > 0 && (dx || part)) {
-        const int vec = vector_of(q, dy, dx);
-        const RopeGrid g = split_of(d, q, vec);
-        if (vec == 4)
-            grid = q->interleaved ? launch_bwd<4, 1, true>(d, q, g, dy, dx, acc_x, part)
-                                  : launch_bwd<4, 1, false>(d, q, g, dy, dx, acc_x, part);
-        else if (vec == 2)
-            grid = q->interleaved ? launch_bwd<2, 2, true>(d, q, g, dy, dx, acc_x, part)
-                                  : launch_bwd<2, 2, false>(d, q, g, dy, dx, acc_x, part);
-        else
-            grid = q->interleaved ? launch_bwd<1, 4, true>(d, q, g, dy, dx, acc_x, part)
-                                  : launch_bwd<1, 4, false>(d, q, g, dy, dx, acc_x, part);
-    }
+    if (n > 0 && (dx || part))
+        grid = q->interleaved ? dispatch<true>(d, q, nullptr, dy, dx, acc_x, part)
+                              : dispatch<false>(d, q, nullptr, dy, dx, acc_x, part);
     if (!part) return;
-    k_rope_dw<<<(2 * q->D + 31) / 32, 256, 0, NCK_STREAM(d)>>>(part, grid, q->D, dwq, acc_q, dwk, acc_k);
+    cudaLaunchAttribute early;
+    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    early.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = (2 * q->D + 31) / 32, cfg.blockDim = 1024, cfg.stream = NCK_STREAM(d);
+    cfg.attrs = &early, cfg.numAttrs = grid > 0;
+    cudaLaunchKernelEx(&cfg, k_rope_dw, (const float *)part, grid, q->D, dwq, acc_q, dwk, acc_k);
     NCK_LAUNCHED(d, 1);
 }

@@ -374,8 +374,8 @@ void nck_rows_bwd(nck_dev *d, const nck_rows *q, const nck_rows_grad *g);
 #define NCK_ROPE_MAX_DIM 256
 /* x [B, T, H, D] by element strides (the last is 1); y, dy and dx are contiguous. Heads below HQ take wq,
  * the others wk (NULL: no weight). Position of axis a at token (b, t): pos[b * pos_b + t * pos_t + a], or t
- * when pos is NULL. Pair i is (i, D/2 + i), or (2i, 2i + 1) when interleaved; it turns turns[i] (in whole
- * turns) per step of axis[i]. */
+ * when pos is NULL. Pair i is (i, D/2 + i), or (2i, 2i + 1) when interleaved; it turns turns[i] (in 2^-64
+ * turns, whole turns left out) per step of axis[i]. */
 typedef struct {
     const float *x;
     int64_t sb, st, sh;
@@ -386,7 +386,7 @@ typedef struct {
     int H, HQ, D, n_axes;
     float eps;
     int norm, interleaved;
-    double turns[NCK_ROPE_MAX_DIM / 2];
+    uint64_t turns[NCK_ROPE_MAX_DIM / 2];
     unsigned char axis[NCK_ROPE_MAX_DIM / 2];
 } nck_rope;
 void nck_rope_fwd(nck_dev *d, const nck_rope *q, float *y);

@@ -28,7 +28,8 @@ static nc_status rope_infer(nc_node *n, nc_dtype *dt, int *nd, int64_t *shape) {
     if (x->ndim != 4) return refuse(ctx, NC_ERR_SHAPE, "x must be [batch, tokens, heads, dim]");
     const int64_t H = x->shape[2], D = x->shape[3], A = n->p.i[P_AXES];
     if (D < 2 || D > NCK_ROPE_MAX_DIM || (D & 1)) return refuse(ctx, NC_ERR_SHAPE, "the head size must be even, 2 to 256");
-    if (H > INT32_MAX || x->shape[1] > INT32_MAX) return refuse(ctx, NC_ERR_SHAPE, "too many heads or tokens");
+    if (H > 65535 || x->shape[0] * x->shape[1] > INT32_MAX - 64)
+        return refuse(ctx, NC_ERR_SHAPE, "more than 65535 heads, or batch * tokens above 2^31 - 65");
     if (n->p.i[P_QHEADS] < 0 || n->p.i[P_QHEADS] > H) return refuse(ctx, NC_ERR_ARG, "q_heads must lie in [0, heads]");
     if (A < 1 || A > 3) return refuse(ctx, NC_ERR_ARG, "n_axes must be 1, 2 or 3");
     int64_t pairs = 0;
@@ -86,14 +87,15 @@ static int rope_of(const nc_node *n, nck_rope *q) {
     q->pos_b = pos && pos->ndim == 3 ? q->T * q->n_axes : 0;
     if (!q->x || (wq && !q->wq) || (wk && !q->wk) || (pos && !q->pos)) return 0;
     /* turns of pair i per step: base^-(i / half) / 2 pi, by repeated products of 64-bit mantissas (half an
-     * ulp each); with AXIS_FREQ i counts from the start of its section and half is the section's length */
+     * ulp each), without whole turns; with AXIS_FREQ i counts from the start of its section and half is the
+     * section's length */
     const long double unit = 0.159154943091895335768883763372514362L, ln_base = logl((long double)n->p.f[0]);
     const int half = q->D / 2, by_axis = (n->p.i[P_FLAGS] & NC_EXT_ROPE_AXIS_FREQ) != 0;
     long double f = unit, step = expl(-ln_base / half);
     for (int a = 0, i = 0; a < q->n_axes; a++) {
         const int len = (int)n->p.i[P_SECTION + a];
         if (by_axis && len) f = unit, step = expl(-ln_base / len);
-        for (int j = 0; j < len; j++, i++, f *= step) q->turns[i] = (double)f, q->axis[i] = (unsigned char)a;
+        for (int j = 0; j < len; j++, i++, f *= step) q->turns[i] = (uint64_t)ldexpl(f - floorl(f), 64), q->axis[i] = (unsigned char)a;
     }
     return 1;
 }
