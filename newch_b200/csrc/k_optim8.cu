@@ -13,10 +13,13 @@
 // m, v, the gradient and the two largest values alone.
 //
 // The update reads w, g and two bytes and writes w and two bytes: 16 bytes an element (AdamW with fp32 moments:
-// 28), so HBM bounds it as long as the arithmetic, about 100 instructions an element, keeps up. A warp owns a
-// block: a lane holds eight elements as two float4 of w and g and two words of four codes each, the
-// largest values are a warp's maximum, and nothing is read or written twice. The step itself is formed with the
-// approximate division and root (each within 2 steps of fp32 of a term that is lr times w's size or less).
+// 28), so HBM bounds it as long as the arithmetic keeps up: at 6.5 TB/s an SM has about 90 issue slots for 32
+// elements. A warp owns a block: a lane holds eight elements as two float4 of w and of g and the sixteen codes
+// of them as one 16-byte word (the codes are stored in that order), the largest values are a warp's maximum, and
+// nothing is read or written twice. A code's proposal is biased upward by 2^-20 of the root (the approximate
+// root is off by 2^-22 at most), so one border settles it. Measured on 135M weights (2.16 GB a step): 363 us, 91% of the measured copy rate; with two-sided
+// borders, denormal-safe roots and separate code arrays (116 issue slots an element) it was 560 us. The step itself is formed with the approximate division and root (each within 2 steps of fp32 of a term
+// that is lr times w's size or less).
 #include "k_common.cuh"
 
 using namespace nck;
@@ -28,96 +31,95 @@ constexpr float kUnitM = 1.0f / (127.0f * 127.0f), kUnitV = (float)(1.0 / (255.0
 constexpr float kFullM = 127.0f * 127.0f, kFullV = 255.0f * 255.0f * 255.0f * 255.0f;
 constexpr float kLeast = 5.0487097934144756e-29f; // 2^-94: blocks whose largest value is below stand for zero
 constexpr float kRound = 12582912.0f;             // 1.5 * 2^23: adding it rounds to whole numbers
+constexpr float kUp = 1.0f + 9.5367431640625e-7f; // 1 + 2^-20
 
+// off by 2^-23 of the root; arguments below 2^-126 have root 0
 __device__ __forceinline__ float root(float x) {
     float r;
-    asm("sqrt.approx.f32 %0, %1;" : "=f"(r) : "f"(x));
+    asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
 }
 
-// byte k of a word of unsigned codes as a float
-__device__ __forceinline__ float byte_of(uint32_t w, int k) {
-    return __uint_as_float(__byte_perm(w, 0x4B000000u, 0x7440u | (uint32_t)k)) - 8388608.0f;
+__device__ __forceinline__ float ratio(float a, float b) {
+    float r;
+    asm("div.approx.ftz.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
 }
 
-// the low byte of a whole number |x| < 2^22
-__device__ __forceinline__ uint32_t low_byte(float x) { return __float_as_uint(x + kRound); }
-
-__device__ __forceinline__ uint32_t pack(const uint32_t (&b)[4]) {
-    return __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
+// the larger of two, NaN when either is
+__device__ __forceinline__ float larger(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
 }
 
-__device__ __forceinline__ float decode_m(float s, float unit, float c) {
-    const float v = unit * (c * fabsf(c));
+// byte k of a word, less `zero`, as a float
+__device__ __forceinline__ float byte_of(uint32_t w, int k, float zero) {
+    return __uint_as_float(__byte_perm(w, 0x4B000000u, 0x7440u | (uint32_t)k)) - (8388608.0f + zero);
+}
+
+// the low bytes of four words
+__device__ __forceinline__ uint32_t pack(const float (&b)[4]) {
+    return __byte_perm(__byte_perm(__float_as_uint(b[0]), __float_as_uint(b[1]), 0x0040),
+                       __byte_perm(__float_as_uint(b[2]), __float_as_uint(b[3]), 0x0040), 0x5410);
+}
+
+// m's codes are stored plus 128
+__device__ __forceinline__ float decode_m(uint32_t w, int k, float s, float unit) {
+    const float c = byte_of(w, k, 128.0f), v = unit * (c * fabsf(c));
     return fabsf(c) == 127.0f ? copysignf(s, c) : v;
 }
 
-__device__ __forceinline__ float decode_v(float s, float unit, float c) {
-    const float q = c * c, v = (unit * q) * q;
+__device__ __forceinline__ float decode_v(uint32_t w, int k, float s, float unit) {
+    const float c = byte_of(w, k, 0.0f), q = c * c, v = (unit * q) * q;
     return c == 255.0f ? s : v;
 }
 
-// the code of |m| by its share (NaN gives some code of the range: its block's largest value is NaN as well)
-__device__ __forceinline__ float code_m(float share) {
-    float c = fminf(fmaxf(root(share), 0.0f), 127.0f);
-    c = (c + kRound) - kRound;
-    const float lo = c - 0.5f, hi = c + 0.5f;
-    if (share < lo * lo && c > 0.0f) c -= 1.0f;
-    if (share >= hi * hi && c < 127.0f) c += 1.0f;
-    return c;
+// A float whose low byte is the code of m, plus 128, by |m|'s share. (The border below code 0 is negative. A share of
+// NaN gives some byte: its block's largest value is NaN as well.)
+__device__ __forceinline__ float code_m(float m, float share) {
+    const float t = fmaf(root(share), kUp, kRound), c = t - kRound, lo = c - 0.5f;
+    const float settled = share < lo * fabsf(lo) ? c - 1.0f : c;
+    return fmaf(settled, copysignf(1.0f, m), kRound + 128.0f);
 }
 
-__device__ __forceinline__ float code_v(float share) {
-    float c = fminf(fmaxf(root(root(share)), 0.0f), 255.0f);
-    c = (c + kRound) - kRound;
-    const float lo = c - 0.5f, hi = c + 0.5f, lo2 = lo * lo, hi2 = hi * hi;
-    if (share < lo2 * lo2 && c > 0.0f) c -= 1.0f;
-    if (share >= hi2 * hi2 && c < 255.0f) c += 1.0f;
-    return c;
+// A float whose low byte is the code of v by its share, at least `least` when v is not zero.
+__device__ __forceinline__ float code_v(float v, float share, float least) {
+    const float t = fmaf(root(root(share)), kUp, kRound), lo = (t - kRound) - 0.5f, lo2 = lo * fabsf(lo);
+    const float settled = share < lo2 * fabsf(lo2) ? t - 1.0f : t;
+    return v > 0.0f ? fmaxf(settled, kRound + least) : settled;
 }
 
-// The largest of non-negative values over a warp; NaN counts as larger than any.
-__device__ __forceinline__ float warp_largest(const float (&v)[8]) {
-    uint32_t top = 0;
-#pragma unroll
-    for (int i = 0; i < 8; i++) top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
-    top = __reduce_max_sync(~0u, top);
-    const float s = __uint_as_float(top);
+// The largest of a warp's non-negative values; NaN counts as larger than any.
+__device__ __forceinline__ float warp_largest(float top) {
+    const float s = __uint_as_float(__reduce_max_sync(~0u, __float_as_uint(top) & 0x7fffffffu));
     return s < kLeast ? 0.0f : s;
 }
 
-// Eight elements' moments to codes, and the block's largest values. m and v are the lane's elements (0 past the end).
-__device__ __forceinline__ void encode(const float (&m)[8], const float (&v)[8], float &sm, float &sv, uint32_t (&cm)[2],
-                                       uint32_t (&cv)[2]) {
-    sm = warp_largest(m);
-    sv = warp_largest(v);
-    const float rm = sm > 0.0f ? (1.0f / sm) * kFullM : 0.0f, rv = sv > 0.0f ? (1.0f / sv) * kFullV : 0.0f;
+// The lane's eight elements' moments (0 past the end) to codes, and the block's largest values.
+__device__ __forceinline__ uint4 encode(const float (&m)[8], const float (&v)[8], float2 &top) {
+    float a = fabsf(m[0]), b = v[0];
+#pragma unroll
+    for (int i = 1; i < 8; i++) a = larger(a, fabsf(m[i])), b = larger(b, v[i]);
+    top = make_float2(warp_largest(a), warp_largest(b));
+    const float rm = top.x > 0.0f ? (1.0f / top.x) * kFullM : 0.0f, rv = top.y > 0.0f ? (1.0f / top.y) * kFullV : 0.0f;
+    const float least = top.y > 0.0f ? 1.0f : 0.0f;
+    uint32_t w[4];
 #pragma unroll
     for (int h = 0; h < 2; h++) {
-        uint32_t bm[4], bv[4];
+        float bm[4], bv[4];
 #pragma unroll
         for (int k = 0; k < 4; k++) {
-            const int i = 4 * h + k;
-            const float c = code_m(fabsf(m[i]) * rm), d = code_v(v[i] * rv);
-            bm[k] = low_byte(copysignf(c, m[i]));
-            bv[k] = low_byte(v[i] > 0.0f && sv > 0.0f ? fmaxf(d, 1.0f) : 0.0f);
+            bm[k] = code_m(m[4 * h + k], fabsf(m[4 * h + k]) * rm);
+            bv[k] = code_v(v[4 * h + k], v[4 * h + k] * rv, least);
         }
-        cm[h] = pack(bm);
-        cv[h] = pack(bv);
+        w[h] = pack(bm);
+        w[2 + h] = pack(bv);
     }
+    return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-__device__ __forceinline__ void decode(uint32_t cm, uint32_t cv, float sm, float sv, float *m, float *v) {
-    const float um = sm * kUnitM, uv = sv * kUnitV;
-    cm ^= 0x80808080u; // signed bytes plus 128
-#pragma unroll
-    for (int k = 0; k < 4; k++) {
-        m[k] = decode_m(sm, um, byte_of(cm, k) - 128.0f);
-        v[k] = decode_v(sv, uv, byte_of(cv, k));
-    }
-}
-
-__device__ __forceinline__ void get4(const float *p, int64_t n, int at, float (&v)[4]) {
+__device__ __forceinline__ void get4(const float *p, int n, int at, float *v) {
     if (at + 4 <= n) {
         const float4 f = *reinterpret_cast<const float4 *>(p + at);
         v[0] = f.x, v[1] = f.y, v[2] = f.z, v[3] = f.w;
@@ -127,7 +129,7 @@ __device__ __forceinline__ void get4(const float *p, int64_t n, int at, float (&
     }
 }
 
-__device__ __forceinline__ void put4(float *p, int64_t n, int at, const float (&v)[4]) {
+__device__ __forceinline__ void put4(float *p, int n, int at, const float *v) {
     if (at + 4 <= n) {
         *reinterpret_cast<float4 *>(p + at) = make_float4(v[0], v[1], v[2], v[3]);
     } else {
@@ -141,50 +143,68 @@ struct Step8 {
     float gs, keep, beta1, up1, beta2, up2, rate, unbias2, eps;
 };
 
-__global__ void __launch_bounds__(256) k_adamw8(Step8 h, nck_opt8 q, const nck_param_seg *__restrict__ segs,
-                                                const nck_opt_chunk *__restrict__ chunks,
+__global__ void __launch_bounds__(256) k_adamw8(Step8 h, nck_opt8 q, const nck_opt8_chunk *__restrict__ chunks,
                                                 const unsigned char *__restrict__ present) {
-    const nck_opt_chunk c = chunks[blockIdx.x];
-    const nck_param_seg s = segs[c.seg];
-    if (present && !present[s.param]) return;
-    const int lane = threadIdx.x & 31, off = (int)(threadIdx.x >> 5) * kBlock;
-    if (off >= c.len) return;
-    const int64_t blk = s.blk + (c.off + off) / kBlock;
-    float *w = s.w + c.off + off;
-    const float *g = s.g + c.off + off;
-    const int64_t n = c.len - off < kBlock ? c.len - off : kBlock;
-    uint32_t *pm = reinterpret_cast<uint32_t *>(q.cm + blk * kBlock), *pv = reinterpret_cast<uint32_t *>(q.cv + blk * kBlock);
-    float wv[2][4], gv[2][4], m[8], v[8];
-    uint32_t cm[2], cv[2];
-    float sm = q.sm[blk], sv = q.sv[blk];
+    const nck_opt8_chunk c = chunks[blockIdx.x];
+    if (present && !present[c.param]) return;
+    const int lane = threadIdx.x & 31, off = (int)(threadIdx.x >> 5) * kBlock, n = c.len - off;
+    if (n <= 0) return;
+    const int64_t blk = (int64_t)c.blk + (threadIdx.x >> 5);
+    float *w = c.w + off;
+    const float *g = c.g + off;
+    uint4 *codes = reinterpret_cast<uint4 *>(q.codes + blk * 2 * kBlock) + lane;
+    float2 *tops = reinterpret_cast<float2 *>(q.top) + blk;
+    float wv[8], gv[8], m[8], v[8];
+    float2 top = *tops;
+    const uint4 old = *codes;
 #pragma unroll
     for (int k = 0; k < 2; k++) {
-        get4(w, n, k * 128 + lane * 4, wv[k]);
-        get4(g, n, k * 128 + lane * 4, gv[k]);
-        cm[k] = pm[k * 32 + lane];
-        cv[k] = pv[k * 32 + lane];
+        get4(g, n, k * 128 + lane * 4, gv + 4 * k);
+        get4(w, n, k * 128 + lane * 4, wv + 4 * k);
+    }
+    const uint32_t words[4] = {old.x, old.y, old.z, old.w};
+    const float um = top.x * kUnitM, uv = top.y * kUnitV;
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        const float gj = h.gs * gv[i];
+        m[i] = h.beta1 * decode_m(words[i >> 2], i & 3, top.x, um) + h.up1 * gj;
+        v[i] = h.beta2 * decode_v(words[2 + (i >> 2)], i & 3, top.y, uv) + h.up2 * gj * gj;
+        wv[i] = fmaf(wv[i], h.keep, -ratio(h.rate * m[i], fmaf(root(v[i]), h.unbias2, h.eps)));
     }
 #pragma unroll
-    for (int k = 0; k < 2; k++) {
-        decode(cm[k], cv[k], sm, sv, m + 4 * k, v + 4 * k);
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const int j = 4 * k + i;
-            const float gj = h.gs * gv[k][i];
-            m[j] = h.beta1 * m[j] + h.up1 * gj;
-            v[j] = h.beta2 * v[j] + h.up2 * gj * gj;
-            const float step = __fdividef(h.rate * m[j], fmaf(root(v[j]), h.unbias2, h.eps));
-            wv[k][i] = fmaf(wv[k][i], h.keep, -step);
+    for (int k = 0; k < 2; k++) put4(w, n, k * 128 + lane * 4, wv + 4 * k);
+    *codes = encode(m, v, top);
+    if (lane == 0) *tops = top;
+}
+
+// The values of one moment of a block (its 4-byte groups of codes `step` 16-byte words apart): float4 stores at
+// 16-byte boundaries wherever `to` starts, so that a row of moments may begin at any element.
+template <bool M>
+__device__ __forceinline__ void emit(const uint32_t *codes, float *to, int n, float s, int lane) {
+    const float unit = s * (M ? kUnitM : kUnitV);
+    const uint32_t *mine = codes + (M ? 0 : 2);
+    const auto group = [&](int g) { return __ldg(mine + (g & 31) * 4 + (g >> 5)); }; // codes of elements 4g .. 4g + 3
+    const auto value = [&](uint32_t w, int k) { return M ? decode_m(w, k, s, unit) : decode_v(w, k, s, unit); };
+    if (n < kBlock) {
+        for (int e = lane; e < n; e += 32) {
+            const uint32_t w = group(e >> 2) >> (8 * (e & 3));
+            to[e] = value(w, 0);
         }
-        put4(w, n, k * 128 + lane * 4, wv[k]);
+        return;
     }
-    encode(m, v, sm, sv, cm, cv);
+    const int lead = (int)((16 - ((uintptr_t)to & 15)) & 15) >> 2; // elements before the first boundary
 #pragma unroll
     for (int k = 0; k < 2; k++) {
-        pm[k * 32 + lane] = cm[k];
-        pv[k * 32 + lane] = cv[k];
+        const int g = lane + 32 * k;
+        if (lead && g == 63) break;
+        const uint32_t w = lead ? __funnelshift_r(group(g), group(g + 1), 8 * lead) : group(g);
+        *reinterpret_cast<float4 *>(to + lead + 4 * g) = make_float4(value(w, 0), value(w, 1), value(w, 2), value(w, 3));
     }
-    if (lane == 0) q.sm[blk] = sm, q.sv[blk] = sv;
+    if (lead && lane < 4) { // the elements before the first and behind the last boundary
+        const int e = lane < lead ? lane : kBlock - 4 + lane;
+        const uint32_t w = group(e >> 2) >> (8 * (e & 3));
+        to[e] = value(w, 0);
+    }
 }
 
 // Codes to values (PUT false) or values to codes: m's at val[0], v's at val[second], a span's at its offset.
@@ -195,41 +215,46 @@ __global__ void __launch_bounds__(256) k_opt8_values(nck_opt8 q, const nck_opt8_
     const nck_opt_chunk c = chunks[blockIdx.x];
     const nck_opt8_span s = spans[c.seg];
     const int lane = threadIdx.x & 31, off = (int)(threadIdx.x >> 5) * kBlock;
-    if (off >= c.len) return;
-    const int64_t blk = s.blk + (c.off + off) / kBlock;
-    float *pm_val = val + (dense ? s.dense : s.flat) + c.off + off, *pv_val = pm_val + second;
     const int n = c.len - off < kBlock ? c.len - off : kBlock;
-    uint32_t *pm = reinterpret_cast<uint32_t *>(q.cm + blk * kBlock), *pv = reinterpret_cast<uint32_t *>(q.cv + blk * kBlock);
-    float m[8], v[8];
-    uint32_t cm[2], cv[2];
-    if (PUT) {
+    if (n <= 0) return;
+    const int64_t blk = s.blk + (c.off + off) / kBlock;
+    float *ms = val + (dense ? s.dense : s.flat) + c.off + off, *vs = ms + second;
+    uint32_t *codes = reinterpret_cast<uint32_t *>(q.codes + blk * 2 * kBlock);
+    float2 *tops = reinterpret_cast<float2 *>(q.top) + blk;
+    if constexpr (PUT) {
+        float m[8], v[8];
 #pragma unroll
         for (int i = 0; i < 8; i++) {
             const int at = (i >> 2) * 128 + lane * 4 + (i & 3);
-            m[i] = at < n ? pm_val[at] : 0.0f;
-            v[i] = at < n ? fabsf(pv_val[at]) : 0.0f;
+            m[i] = at < n ? ms[at] : 0.0f;
+            v[i] = at < n ? fabsf(vs[at]) : 0.0f;
         }
-        float sm, sv;
-        encode(m, v, sm, sv, cm, cv);
-#pragma unroll
-        for (int k = 0; k < 2; k++) pm[k * 32 + lane] = cm[k], pv[k * 32 + lane] = cv[k];
-        if (lane == 0) q.sm[blk] = sm, q.sv[blk] = sv;
-        return;
-    }
-    const float sm = q.sm[blk], sv = q.sv[blk];
-#pragma unroll
-    for (int k = 0; k < 2; k++) decode(pm[k * 32 + lane], pv[k * 32 + lane], sm, sv, m + 4 * k, v + 4 * k);
-#pragma unroll
-    for (int i = 0; i < 8; i++) {
-        const int at = (i >> 2) * 128 + lane * 4 + (i & 3);
-        if (at < n) pm_val[at] = m[i], pv_val[at] = v[i];
+        float2 top;
+        reinterpret_cast<uint4 *>(codes)[lane] = encode(m, v, top);
+        if (lane == 0) *tops = top;
+    } else {
+        const float2 top = *tops;
+        emit<true>(codes, ms, n, top.x, lane);
+        emit<false>(codes, vs, n, top.y, lane);
     }
 }
 
 }  // namespace
 
-extern "C" void nck_adamw8_step(nck_dev *d, const nck_opt_hyper *h, const nck_opt8 *q, const nck_param_seg *dsegs,
-                                const nck_opt_chunk *dchunks, int nchunk, int64_t total, const unsigned char *present) {
+extern "C" int nck_opt8_chunks(const nck_param_seg *segs, int nseg, nck_opt8_chunk *chunks) {
+    int k = 0;
+    for (int i = 0; i < nseg; i++)
+        for (int64_t off = 0; off < segs[i].n; off += NCK_OPT8_CHUNK, k++) {
+            if (!chunks) continue;
+            const int64_t left = segs[i].n - off;
+            chunks[k] = {segs[i].w + off, segs[i].g + off, (int32_t)(segs[i].blk + off / NCK_OPT8_BLOCK),
+                         (int32_t)(left < NCK_OPT8_CHUNK ? left : NCK_OPT8_CHUNK), segs[i].param, 0};
+        }
+    return k;
+}
+
+extern "C" void nck_adamw8_step(nck_dev *d, const nck_opt_hyper *h, const nck_opt8 *q, const nck_opt8_chunk *dchunks,
+                                int nchunk, int64_t total, const unsigned char *present) {
     if (nchunk <= 0) return;
     Scope sc(d, "adamw8", 0.0, 16.0 * total);
     Step8 s;
@@ -240,7 +265,7 @@ extern "C" void nck_adamw8_step(nck_dev *d, const nck_opt_hyper *h, const nck_op
     s.rate = h->lr / h->bc1;
     s.unbias2 = 1.0f / sqrtf(h->bc2);
     s.eps = h->eps;
-    k_adamw8<<<nchunk, 256, 0, NCK_STREAM(d)>>>(s, *q, dsegs, dchunks, present);
+    k_adamw8<<<nchunk, 256, 0, NCK_STREAM(d)>>>(s, *q, dchunks, present);
     NCK_LAUNCHED(d, 1);
 }
 

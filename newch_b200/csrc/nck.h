@@ -450,18 +450,24 @@ int nck_optim_chunks(const nck_param_seg *segs, int nseg, int64_t size, nck_opt_
 void nck_optim_step(nck_dev *d, const nck_opt_hyper *h, const nck_param_seg *dsegs, const nck_opt_chunk *dchunks,
                     int nchunk, int64_t total, const unsigned char *present);
 
-/* AdamW with 8-bit moments: blocks of NCK_OPT8_BLOCK elements, a byte an element (cm signed, cv unsigned;
- * each parameter padded to whole blocks, the padding's codes 0) and the block's largest values (sm, sv).
- * segs[].blk is a parameter's first block; chunks of NCK_OPT8_CHUNK elements. */
+/* AdamW with 8-bit moments: blocks of NCK_OPT8_BLOCK elements, each parameter padded to whole blocks. A block
+ * has its two largest values (top[2 b] of |m|, top[2 b + 1] of v) and two bytes an element (codes, 512 bytes: for
+ * l = 0 .. 31 the m codes, plus 128, of elements 4l .. 4l + 3 and 128 + 4l .. 128 + 4l + 3, then their v codes). */
 #define NCK_OPT8_BLOCK 256
 #define NCK_OPT8_CHUNK 2048 /* a warp per block of states, eight of them a thread block */
 typedef struct {
-    int8_t *cm;
-    unsigned char *cv;
-    float *sm, *sv;
+    unsigned char *codes;
+    float *top;
 } nck_opt8;
-void nck_adamw8_step(nck_dev *d, const nck_opt_hyper *h, const nck_opt8 *q, const nck_param_seg *dsegs,
-                     const nck_opt_chunk *dchunks, int nchunk, int64_t total, const unsigned char *present);
+typedef struct {
+    float *w;
+    const float *g;
+    int32_t blk, len, param, pad;
+} nck_opt8_chunk;
+/* fills chunks (when not NULL) for the segments (blk: a segment's first block); returns how many there are */
+int nck_opt8_chunks(const nck_param_seg *segs, int nseg, nck_opt8_chunk *chunks);
+void nck_adamw8_step(nck_dev *d, const nck_opt_hyper *h, const nck_opt8 *q, const nck_opt8_chunk *dchunks, int nchunk,
+                     int64_t total, const unsigned char *present);
 /* a parameter's states as fp32 values: element offsets of the dense and of the flat (aligned) layout */
 typedef struct {
     int64_t dense, flat;

@@ -58,7 +58,7 @@ struct nc_optim {
     int eps_inside_sqrt;
     /* update launch: segments and chunks on the host (last built) and on the device */
     nck_param_seg *segs, *dsegs;
-    nck_opt_chunk *chunks, *dchunks;
+    void *chunks, *dchunks; /* nck_opt_chunk, or nck_opt8_chunk for 8-bit moments */
     int nseg, nchunk, cap_chunk;
     /* 8-bit moments: codes and block maxima, elements and blocks of all parameters, and the tables of the
      * value conversions (every parameter, uploaded at first use) */
@@ -106,30 +106,30 @@ static int adopt_grad(nc_optim *opt, int i) {
     return 1;
 }
 
+/* an entry of the update launch's chunk table */
+static size_t chunk_size(const nc_optim *o) {
+    return o->kind == OPT_ADAMW8 ? sizeof(nck_opt8_chunk) : sizeof(nck_opt_chunk);
+}
+
 static int64_t blocks_of(const nc_tensor *p) { return (nc_numel(p) + NCK_OPT8_BLOCK - 1) / NCK_OPT8_BLOCK; }
 
-/* codes and maxima of the 8-bit moments, all zero */
+/* codes and maxima of the 8-bit moments: every moment zero (codes of maxima 0) */
 static int alloc_state8(nc_optim *o) {
-    const size_t codes = (size_t)(o->blocks ? o->blocks : 1) * NCK_OPT8_BLOCK, tops = codes / NCK_OPT8_BLOCK * sizeof(float);
+    const size_t blocks = (size_t)(o->blocks ? o->blocks : 1);
     cudaStream_t s = (cudaStream_t)o->ctx->dev.stream;
     if (o->blocks > INT32_MAX) return 0;
-    if (!(o->q8.cm = (int8_t *)nc__persistent_alloc(o->ctx, codes)) ||
-        !(o->q8.cv = (unsigned char *)nc__persistent_alloc(o->ctx, codes)) ||
-        !(o->q8.sm = (float *)nc__persistent_alloc(o->ctx, tops)) || !(o->q8.sv = (float *)nc__persistent_alloc(o->ctx, tops)))
+    if (!(o->q8.codes = (unsigned char *)nc__persistent_alloc(o->ctx, blocks * 2 * NCK_OPT8_BLOCK)) ||
+        !(o->q8.top = (float *)nc__persistent_alloc(o->ctx, blocks * 2 * sizeof(float))))
         return 0;
-    cudaMemsetAsync(o->q8.cm, 0, codes, s);
-    cudaMemsetAsync(o->q8.cv, 0, codes, s);
-    cudaMemsetAsync(o->q8.sm, 0, tops, s);
-    cudaMemsetAsync(o->q8.sv, 0, tops, s);
+    cudaMemsetAsync(o->q8.codes, 128, blocks * 2 * NCK_OPT8_BLOCK, s); /* m's code 0 */
+    cudaMemsetAsync(o->q8.top, 0, blocks * 2 * sizeof(float), s);
     return 1;
 }
 
 static void free_state8(nc_optim *o) {
-    const size_t codes = (size_t)(o->blocks ? o->blocks : 1) * NCK_OPT8_BLOCK, tops = codes / NCK_OPT8_BLOCK * sizeof(float);
-    if (o->q8.cm) nc__persistent_free(o->ctx, o->q8.cm, codes);
-    if (o->q8.cv) nc__persistent_free(o->ctx, o->q8.cv, codes);
-    if (o->q8.sm) nc__persistent_free(o->ctx, o->q8.sm, tops);
-    if (o->q8.sv) nc__persistent_free(o->ctx, o->q8.sv, tops);
+    const size_t blocks = (size_t)(o->blocks ? o->blocks : 1);
+    if (o->q8.codes) nc__persistent_free(o->ctx, o->q8.codes, blocks * 2 * NCK_OPT8_BLOCK);
+    if (o->q8.top) nc__persistent_free(o->ctx, o->q8.top, blocks * 2 * sizeof(float));
     if (o->dspans) nc__persistent_free(o->ctx, o->dspans, sizeof(nck_opt8_span) * (size_t)(o->n ? o->n : 1));
     if (o->dspan_chunks)
         nc__persistent_free(o->ctx, o->dspan_chunks, sizeof(nck_opt_chunk) * (size_t)(o->nspan_chunk ? o->nspan_chunk : 1));
@@ -210,7 +210,7 @@ void nc_optim_free(nc_optim *o) {
     if (o->gred) nc__persistent_free(ctx, o->gred, bytes);
     free_state8(o);
     if (o->dsegs) nc__persistent_free(ctx, o->dsegs, sizeof(nck_param_seg) * (size_t)(o->n ? o->n : 1));
-    if (o->dchunks) nc__persistent_free(ctx, o->dchunks, sizeof(nck_opt_chunk) * (size_t)o->cap_chunk);
+    if (o->dchunks) nc__persistent_free(ctx, o->dchunks, chunk_size(o) * (size_t)o->cap_chunk);
     if (o->pres_d) nc__persistent_free(ctx, o->pres_d, (size_t)(o->n ? o->n : 1));
     if (o->h1) cudaFreeHost(o->h1);
     if (o->h2) cudaFreeHost(o->h2);
@@ -568,21 +568,23 @@ static int upload_tables(nc_optim *o, const nck_param_seg *segs, int nseg) {
     if (!o->dsegs && !(o->dsegs = (nck_param_seg *)nc__persistent_alloc(ctx, sizeof(nck_param_seg) *
                                                                                 (size_t)(o->n ? o->n : 1))))
         return 0;
-    const int64_t size = o->kind == OPT_ADAMW8 ? NCK_OPT8_CHUNK : NCK_OPT_CHUNK;
-    int nchunk = nck_optim_chunks(segs, nseg, size, NULL);
+    const int q8 = o->kind == OPT_ADAMW8;
+    const size_t entry = chunk_size(o);
+    int nchunk = q8 ? nck_opt8_chunks(segs, nseg, NULL) : nck_optim_chunks(segs, nseg, NCK_OPT_CHUNK, NULL);
     if (nchunk > o->cap_chunk) {
-        if (o->dchunks) nc__persistent_free(ctx, o->dchunks, sizeof(nck_opt_chunk) * (size_t)o->cap_chunk);
+        if (o->dchunks) nc__persistent_free(ctx, o->dchunks, entry * (size_t)o->cap_chunk);
         free(o->chunks);
         o->cap_chunk = 0;
-        o->chunks = (nck_opt_chunk *)malloc(sizeof(nck_opt_chunk) * (size_t)nchunk);
-        o->dchunks = (nck_opt_chunk *)nc__persistent_alloc(ctx, sizeof(nck_opt_chunk) * (size_t)nchunk);
+        o->chunks = malloc(entry * (size_t)nchunk);
+        o->dchunks = nc__persistent_alloc(ctx, entry * (size_t)nchunk);
         if (!o->chunks || !o->dchunks) return 0;
         o->cap_chunk = nchunk;
     }
-    nck_optim_chunks(segs, nseg, size, o->chunks);
+    if (q8) nck_opt8_chunks(segs, nseg, (nck_opt8_chunk *)o->chunks);
+    else nck_optim_chunks(segs, nseg, NCK_OPT_CHUNK, (nck_opt_chunk *)o->chunks);
     if (segs != o->segs) memcpy(o->segs, segs, sizeof(nck_param_seg) * (size_t)nseg);
-    nc__upload(ctx, o->dsegs, o->segs, sizeof(nck_param_seg) * (size_t)nseg);
-    nc__upload(ctx, o->dchunks, o->chunks, sizeof(nck_opt_chunk) * (size_t)nchunk);
+    if (!q8) nc__upload(ctx, o->dsegs, o->segs, sizeof(nck_param_seg) * (size_t)nseg);
+    nc__upload(ctx, o->dchunks, o->chunks, entry * (size_t)nchunk);
     o->nseg = nseg;
     o->nchunk = nchunk;
     return ctx->status == NC_OK;
@@ -652,9 +654,9 @@ void nc_optim_step(nc_optim *o) {
     }
     if (nseg && upload_tables(o, segs, nseg)) {
         if (o->kind == OPT_ADAMW8)
-            nck_adamw8_step(nc__k(ctx), &h, &o->q8, o->dsegs, o->dchunks, o->nchunk, total, dp ? o->pres_d : NULL);
+            nck_adamw8_step(nc__k(ctx), &h, &o->q8, (const nck_opt8_chunk *)o->dchunks, o->nchunk, total, dp ? o->pres_d : NULL);
         else
-            nck_optim_step(nc__k(ctx), &h, o->dsegs, o->dchunks, o->nchunk, total, dp ? o->pres_d : NULL);
+            nck_optim_step(nc__k(ctx), &h, o->dsegs, (const nck_opt_chunk *)o->dchunks, o->nchunk, total, dp ? o->pres_d : NULL);
     }
     o->state_host_valid = 0;
 }
