@@ -7,10 +7,14 @@
 // 4 bytes a logit forward, 8 backward, about one exponential each, so HBM bounds them. Rows that the mask leaves
 // out are not read; their gradient is zeros.
 //
-// A row of up to kWarpRow logits belongs to a warp, a longer one to a block of 256 threads. A warp takes a
-// run of up to 32 rows and keeps the statistics of row i in lane i, so that the double precision arithmetic of
-// the loss runs once a run and not once a row. Log probabilities and everything behind them that can cancel
-// (log ratios, sums over tokens and rows) are held in 64 bits; sums run in a fixed order.
+// A row of up to kWarpRow logits belongs to a warp, a longer one to a block of 256 threads with many loads in
+// flight a thread (8 vectors forward, 16 backward: 4 x 2048 rows of 50001 logits with half of the rows counted take
+// 123 and 354 us, 0.82 and 2.46 GB at the copy rate 125 and 375; with 4 vectors 128 and 376). A few very long
+// rows are split among warps, and a second launch joins the parts. Statistics of up to 32 rows wait in a warp's lanes,
+// so that the double precision arithmetic of the loss runs once for all of them and not once a row. Backward has a
+// block a row (uncounted rows cost a third, so dealing rows out in advance leaves SMs idle: 418 us) and starts with
+// the last row, whose logits the forward pass may have left in L2. Log probabilities and everything behind them that
+// can cancel (log ratios, sums over tokens and rows) are held in 64 bits; sums run in a fixed order.
 #include <math.h>
 
 #include "k_common.cuh"
@@ -22,6 +26,13 @@ namespace {
 constexpr int kWarpRow = 1024;
 constexpr float kNone = -INFINITY;
 
+// e^x by the approximate power of two: off by 2 steps and the rounding of x log2 e; results below 2^-126 are 0
+__device__ __forceinline__ float exp_of(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x * 1.4426950408889634f));
+    return r;
+}
+
 struct Stat {
     float m, s; // running maximum, and the sum of exp(z - m)
 };
@@ -29,7 +40,7 @@ struct Stat {
 // adds a maximum / sum pair to another; a side without finite values has s = 0
 __device__ __forceinline__ Stat join(Stat a, Stat b) {
     const float m = fmaxf(a.m, b.m), base = m == kNone ? 0.0f : m;
-    return {m, a.s * __expf(a.m - base) + b.s * __expf(b.m - base)};
+    return {m, a.s * exp_of(a.m - base) + b.s * exp_of(b.m - base)};
 }
 
 template <int N>
@@ -38,9 +49,9 @@ __device__ __forceinline__ void take(Stat &st, const float (&v)[N]) {
 #pragma unroll
     for (int i = 1; i < N; i++) top = fmaxf(top, v[i]);
     const float m = fmaxf(st.m, top), base = m == kNone ? 0.0f : m;
-    float s = st.s * __expf(st.m - base);
+    float s = st.s * exp_of(st.m - base);
 #pragma unroll
-    for (int i = 0; i < N; i++) s += __expf(v[i] - base);
+    for (int i = 0; i < N; i++) s += exp_of(v[i] - base);
     st.m = m, st.s = s;
 }
 
@@ -50,23 +61,38 @@ __device__ __forceinline__ int64_t lead_of(const float *p, int64_t n) {
     return k < n ? k : n;
 }
 
-// A team of W threads (t of them) reads a row: U vectors in flight each.
+// Vectors before part k of n of a row's nv (V < 2^31, so nv < 2^29, and there are at most nv / 8 parts).
+__device__ __forceinline__ int part_begin(int nv, int k, int n) { return n == 1 ? (k ? nv : 0) : (int)((int64_t)nv * k / n); }
+
+// A team of W threads (t of them) reads part k of n of a row: U vectors in flight each.
 template <int W, int U>
-__device__ __forceinline__ Stat read_row(const float *z, int64_t V, int t) {
+__device__ __forceinline__ Stat read_row(const float *z, int64_t V, int t, int k, int n) {
     Stat st = {kNone, 0.0f};
-    const int64_t lead = lead_of(z, V), nv = (V - lead) >> 2;
+    const int64_t lead = lead_of(z, V);
+    const int nv = (int)((V - lead) >> 2), end = part_begin(nv, k + 1, n);
     const float4 *z4 = reinterpret_cast<const float4 *>(z + lead);
-    for (int64_t i = t; i < nv; i += W * U) {
+    int i = part_begin(nv, k, n) + t;
+    for (; i + (U - 1) * W < end; i += W * U) {
+        float4 f[U];
         float v[4 * U];
 #pragma unroll
-        for (int u = 0; u < U; u++) {
-            float4 f = make_float4(kNone, kNone, kNone, kNone);
-            if (i + u * W < nv) f = __ldg(z4 + i + u * W);
-            v[4 * u] = f.x, v[4 * u + 1] = f.y, v[4 * u + 2] = f.z, v[4 * u + 3] = f.w;
-        }
+        for (int u = 0; u < U; u++) f[u] = __ldg(z4 + i + u * W);
+#pragma unroll
+        for (int u = 0; u < U; u++) v[4 * u] = f[u].x, v[4 * u + 1] = f[u].y, v[4 * u + 2] = f[u].z, v[4 * u + 3] = f[u].w;
         take(st, v);
     }
-    const int64_t tail = lead + 4 * nv;
+    if (i < end) { // the rest, at most U - 1 vectors a thread
+        float4 f[U - 1 > 0 ? U - 1 : 1];
+#pragma unroll
+        for (int u = 0; u < U - 1; u++) f[u] = i + u * W < end ? __ldg(z4 + i + u * W) : make_float4(kNone, kNone, kNone, kNone);
+#pragma unroll
+        for (int u = 0; u < U - 1; u++) {
+            const float v[4] = {f[u].x, f[u].y, f[u].z, f[u].w};
+            if (i + u * W < end) take(st, v);
+        }
+    }
+    if (k) return st; // part 0 has the ends that are no whole vectors
+    const int64_t tail = lead + 4 * (int64_t)nv;
     if (t < lead) {
         const float v[1] = {z[t]};
         take(st, v);
@@ -143,37 +169,43 @@ __device__ __forceinline__ void skip_row(const nck_rows &q, const nck_policy &p,
     if (p.coef) p.coef[r] = 0.0f;
 }
 
-// Loss and 1 / count from every block's sums, in block order, by the block that ends last.
-__device__ void finish_loss(const nck_policy &p, Sums mine, double2 *part, unsigned *counter) {
+// The sums of a block's threads, in thread 0.
+__device__ Sums block_sums(Sums mine) {
     __shared__ double2 red[8];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    for (int round = 0; round < 2; round++) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-            mine.loss += __shfl_xor_sync(~0u, mine.loss, o);
-            mine.count += __shfl_xor_sync(~0u, mine.count, o);
-        }
-        __syncthreads();
-        if (lane == 0) red[warp] = make_double2(mine.loss, mine.count);
-        __syncthreads();
-        Sums all = {0.0, 0.0};
-        for (int w = 0; w < 8; w++) all.loss += red[w].x, all.count += red[w].y;
-        if (round) {
-            if (threadIdx.x == 0) {
-                const double n = all.count > 1.0 ? all.count : 1.0;
-                *p.loss = (float)(all.loss / n);
-                if (p.scale) *p.scale = (float)(1.0 / n);
-            }
-            return;
-        }
-        if (threadIdx.x == 0) part[blockIdx.x] = make_double2(all.loss, all.count);
-        if (!last_block_done(counter)) return;
-        mine = {0.0, 0.0};
-        for (int b = threadIdx.x; b < (int)gridDim.x; b += blockDim.x) {
-            const double2 v = __ldcg(part + b);
-            mine.loss += v.x, mine.count += v.y;
-        }
+    for (int o = 16; o > 0; o >>= 1) {
+        mine.loss += __shfl_xor_sync(~0u, mine.loss, o);
+        mine.count += __shfl_xor_sync(~0u, mine.count, o);
     }
+    __syncthreads();
+    if (lane == 0) red[warp] = make_double2(mine.loss, mine.count);
+    __syncthreads();
+    mine = {0.0, 0.0};
+    if (threadIdx.x == 0)
+        for (int w = 0; w < warps; w++) mine.loss += red[w].x, mine.count += red[w].y;
+    return mine;
+}
+
+// Loss and 1 / count, from thread 0's sums.
+__device__ void write_loss(const nck_policy &p, Sums all) {
+    if (threadIdx.x) return;
+    const double n = all.count > 1.0 ? all.count : 1.0;
+    *p.loss = (float)(all.loss / n);
+    if (p.scale) *p.scale = (float)(1.0 / n);
+}
+
+// The same from every block's sums, in block order, by the block that ends last.
+__device__ void finish_loss(const nck_policy &p, Sums mine, double2 *part, unsigned *counter) {
+    mine = block_sums(mine);
+    if (threadIdx.x == 0) part[blockIdx.x] = make_double2(mine.loss, mine.count);
+    if (!last_block_done(counter)) return;
+    mine = {0.0, 0.0};
+    for (int b = threadIdx.x; b < (int)gridDim.x; b += blockDim.x) {
+        const double2 v = __ldcg(part + b);
+        mine.loss += v.x, mine.count += v.y;
+    }
+    write_loss(p, block_sums(mine));
 }
 
 // One warp a run of `run` rows, row i's statistics in lane i.
@@ -186,10 +218,10 @@ __global__ void __launch_bounds__(256) k_rows_warp(nck_rows q, nck_policy p, int
         const bool live = lane < n && counted(q, r0 + lane);
         const unsigned any = __ballot_sync(~0u, live);
         Stat own = {kNone, 0.0f};
-        for (int i = 0; i < n; i++) {
-            if (!(any >> i & 1)) continue;
-            const Stat st = warp_join(read_row<32, 1>(row_of(q, r0 + i), q.V, lane));
-            if (lane == i) own = st;
+        for (int k = 0; k < n; k++) {
+            if (!(any >> k & 1)) continue;
+            const Stat st = warp_join(read_row<32, 1>(row_of(q, r0 + k), q.V, lane, 0, 1));
+            if (lane == k) own = st;
         }
         if (live) {
             const Sums s = finish_row(q, p, r0 + lane, own);
@@ -201,28 +233,81 @@ __global__ void __launch_bounds__(256) k_rows_warp(nck_rows q, nck_policy p, int
     if (p.loss) finish_loss(p, sums, part, counter);
 }
 
-// One block a row.
+// A block a row. Statistics of counted rows wait in the lanes of the first warp, which finishes 32 at a time.
 __global__ void __launch_bounds__(256) k_rows_block(nck_rows q, nck_policy p, double2 *part, unsigned *counter) {
     __shared__ Stat red[2][8];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     Sums sums = {0.0, 0.0};
-    int turn = 0;
+    Stat own = {kNone, 0.0f};
+    int64_t own_row = -1;
+    int turn = 0, held = 0;
+    const auto finish = [&]() {
+        if (own_row >= 0) {
+            const Sums s = finish_row(q, p, own_row, own);
+            sums.loss += s.loss, sums.count += s.count;
+        }
+        own_row = -1, held = 0;
+    };
     for (int64_t r = blockIdx.x; r < q.N; r += gridDim.x) {
         if (!counted(q, r)) {
             if (threadIdx.x == 0) skip_row(q, p, r);
             continue;
         }
-        const Stat st = warp_join(read_row<256, 4>(row_of(q, r), q.V, threadIdx.x));
-        if ((threadIdx.x & 31) == 0) red[turn][threadIdx.x >> 5] = st;
+        const Stat st = warp_join(read_row<256, 8>(row_of(q, r), q.V, threadIdx.x, 0, 1));
+        if (lane == 0) red[turn][warp] = st;
         __syncthreads();
-        if (threadIdx.x == 0) {
-            Stat all = red[turn][0];
-            for (int w = 1; w < 8; w++) all = join(all, red[turn][w]);
-            const Sums s = finish_row(q, p, r, all);
-            sums.loss += s.loss, sums.count += s.count;
+        if (warp == 0) {
+            Stat all = {kNone, 0.0f};
+            if (lane < 8) all = red[turn][lane];
+            all = warp_join(all);
+            if (lane == held) own = all, own_row = r;
+            if (++held == 32) finish();
         }
         turn ^= 1;
     }
+    if (warp == 0) finish();
     if (p.loss) finish_loss(p, sums, part, counter);
+}
+
+// Few rows: a warp takes parts of rows, with no barrier between warps; k_rows_finish joins them.
+__global__ void __launch_bounds__(256) k_rows_parts(nck_rows q, int parts, float2 *part) {
+    const int lane = threadIdx.x & 31;
+    for (int64_t it = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); it < q.N * parts; it += (int64_t)gridDim.x * 8) {
+        const int64_t r = it / parts;
+        if (!counted(q, r)) continue;
+        const Stat all = warp_join(read_row<32, 4>(row_of(q, r), q.V, lane, (int)(it - r * parts), parts));
+        if (lane == 0) part[it] = make_float2(all.m, all.s);
+    }
+}
+
+// A warp a run of rows: their parts joined, row i's in lane i, and the rows finished.
+__global__ void __launch_bounds__(256) k_rows_finish(nck_rows q, nck_policy p, int parts, int run, const float2 *part,
+                                                     double2 *sums_of, unsigned *counter) {
+    cudaGridDependencySynchronize(); // launched early: the parts are there when the kernel before has ended
+    const int lane = threadIdx.x & 31;
+    Sums sums = {0.0, 0.0};
+    const int64_t r0 = ((int64_t)blockIdx.x * 8 + (threadIdx.x >> 5)) * run;
+    const int n = q.N - r0 < run ? (int)(q.N - r0) : run;
+    const bool live = lane < n && counted(q, r0 + lane);
+    const unsigned any = __ballot_sync(~0u, live);
+    Stat own = {kNone, 0.0f};
+    for (int i = 0; i < n; i++) {
+        if (!(any >> i & 1)) continue;
+        Stat st = {kNone, 0.0f};
+        for (int k = lane; k < parts; k += 32) {
+            const float2 v = __ldcg(part + (r0 + i) * parts + k);
+            st = join(st, {v.x, v.y});
+        }
+        st = warp_join(st);
+        if (lane == i) own = st;
+    }
+    if (live) {
+        const Sums s = finish_row(q, p, r0 + lane, own);
+        sums.loss += s.loss, sums.count += s.count;
+    } else if (lane < n) {
+        skip_row(q, p, r0 + lane);
+    }
+    if (p.loss) finish_loss(p, sums, sums_of, counter);
 }
 
 // Sums of a pair's two sequences, the pair's loss term and its sequences' factors; the last block sums the terms.
@@ -269,78 +354,104 @@ __global__ void __launch_bounds__(256) k_pairs(nck_pairs p, const double *__rest
     }
 }
 
-// The gradient of one row by a team of W threads: dst (+)= c (1[j = a] - exp(z - m) inv).
+// The gradient of part k of n of a row by a team of W threads: dst (+)= c (1[j = a] - exp(z - m) inv).
 template <int W, int U, bool ACC>
-__device__ __forceinline__ void grad_row(const float *z, float *dst, int64_t V, float c, float m, float inv, int64_t a, int t) {
-    if (c == 0.0f) { // nothing of the row is read
-        if (ACC) return;
-        const int64_t lead = lead_of(dst, V), nv = (V - lead) >> 2, tail = lead + 4 * nv;
-        float4 *d4 = reinterpret_cast<float4 *>(dst + lead);
-        for (int64_t i = t; i < nv; i += W) d4[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (t < lead) dst[t] = 0.0f;
-        if (t < V - tail) dst[tail + t] = 0.0f;
-        return;
-    }
+__device__ __forceinline__ void grad_row(const float *z, float *dst, int64_t V, float c, float m, float inv, int64_t a, int t,
+                                         int k, int n) {
+    const bool even = (((uintptr_t)z ^ (uintptr_t)dst) & 15) == 0; // the row and its gradient share their boundaries
+    const bool blank = c == 0.0f;                                  // nothing of the row is read
+    if (ACC && blank) return;
+    const int64_t lead = lead_of(dst, V);
+    const int nv = (int)((V - lead) >> 2), end = part_begin(nv, k + 1, n);
+    const int64_t tail = lead + 4 * (int64_t)nv;
+    float4 *d4 = reinterpret_cast<float4 *>(dst + lead);
     const float f = -c * inv;
     const auto one = [&](int64_t j) {
-        float v = f * __expf(z[j] - m);
+        float v = blank ? 0.0f : f * exp_of(z[j] - m);
         if (j == a) v += c;
         dst[j] = ACC ? dst[j] + v : v;
     };
-    if ((((uintptr_t)z ^ (uintptr_t)dst) & 15) != 0) { // rows of another alignment than their gradient's
-        for (int64_t j = t; j < V; j += W) one(j);
+    if (k == 0) {
+        if (t < lead) one(t);
+        if (t < V - tail) one(tail + t);
+    }
+    int i = part_begin(nv, k, n) + t;
+    if (blank) {
+        for (; i < end; i += W) d4[i] = make_float4(0.f, 0.f, 0.f, 0.f);
         return;
     }
-    const int64_t lead = lead_of(z, V), nv = (V - lead) >> 2, tail = lead + 4 * nv;
-    const float4 *z4 = reinterpret_cast<const float4 *>(z + lead);
-    float4 *d4 = reinterpret_cast<float4 *>(dst + lead);
-    for (int64_t i = t; i < nv; i += W * U) {
-        float4 v[U], old[ACC ? U : 1];
+    const float *from = z + lead;
+    const int64_t hot = a - lead; // the label's place among the vectors' floats
+    const auto fetch = [&](int j) {
+        const float *at = from + 4 * (int64_t)j;
+        return even ? __ldg(reinterpret_cast<const float4 *>(at)) : make_float4(__ldg(at), __ldg(at + 1), __ldg(at + 2), __ldg(at + 3));
+    };
+    const auto give = [&](int j, float4 v, float4 old) {
+        float4 g = make_float4(f * exp_of(v.x - m), f * exp_of(v.y - m), f * exp_of(v.z - m), f * exp_of(v.w - m));
+        const uint64_t w = (uint64_t)(hot - 4 * (int64_t)j);
+        if (w < 4) g.x += w == 0 ? c : 0.0f, g.y += w == 1 ? c : 0.0f, g.z += w == 2 ? c : 0.0f, g.w += w == 3 ? c : 0.0f;
+        if (ACC) g.x += old.x, g.y += old.y, g.z += old.z, g.w += old.w;
+        d4[j] = g;
+    };
+    for (; i < end; i += W * U) {
+        float4 v[U], old[ACC ? U : 1] = {};
 #pragma unroll
         for (int u = 0; u < U; u++)
-            if (i + u * W < nv) {
-                v[u] = __ldg(z4 + i + u * W);
+            if (i + u * W < end) {
+                v[u] = fetch(i + u * W);
                 if (ACC) old[ACC ? u : 0] = d4[i + u * W];
             }
 #pragma unroll
-        for (int u = 0; u < U; u++) {
-            if (i + u * W >= nv) break;
-            float4 g = make_float4(f * __expf(v[u].x - m), f * __expf(v[u].y - m), f * __expf(v[u].z - m), f * __expf(v[u].w - m));
-            const uint64_t k = (uint64_t)(a - lead - 4 * (i + u * W));
-            if (k < 4) g.x += k == 0 ? c : 0.0f, g.y += k == 1 ? c : 0.0f, g.z += k == 2 ? c : 0.0f, g.w += k == 3 ? c : 0.0f;
-            if (ACC) {
-                const float4 o = old[ACC ? u : 0];
-                g.x += o.x, g.y += o.y, g.z += o.z, g.w += o.w;
-            }
-            d4[i + u * W] = g;
-        }
+        for (int u = 0; u < U; u++)
+            if (i + u * W < end) give(i + u * W, v[u], old[ACC ? u : 0]);
     }
-    if (t < lead) one(t);
-    if (t < V - tail) one(tail + t);
 }
 
 template <int W, bool ACC>
-__global__ void __launch_bounds__(256) k_rows_grad(nck_rows q, nck_rows_grad g) {
+__global__ void __launch_bounds__(256) k_rows_grad(nck_rows q, nck_rows_grad g, int parts) {
     const int t = threadIdx.x % W;
     const float up = g.up[0] * (g.scale ? g.scale[0] : 1.0f);
     const int64_t teams = (int64_t)gridDim.x * (256 / W);
-    for (int64_t r = (int64_t)blockIdx.x * (256 / W) + threadIdx.x / W; r < q.N; r += teams) {
+    // from the last row back: what the forward pass read last is still in L2
+    for (int64_t it = (int64_t)blockIdx.x * (256 / W) + threadIdx.x / W; it < q.N * parts; it += teams) {
+        const int64_t turn = parts == 1 ? it : it / parts, r = q.N - 1 - turn;
         const float c = counted(q, r) ? up * g.coef[r / g.per_coef] : 0.0f;
         const float2 st = c == 0.0f ? make_float2(0.f, 0.f) : reinterpret_cast<const float2 *>(q.stat)[r];
         int64_t a = q.lab[r];
         if (a < 0 || a >= q.V) a = 0;
-        grad_row<W, W == 32 ? 1 : 4, ACC>(row_of(q, r), g.dz + r * q.V, q.V, c, st.x, st.y, a, t);
+        grad_row<W, W == 32 ? 1 : ACC ? 8 : 16, ACC>(row_of(q, r), g.dz + r * q.V, q.V, c, st.x, st.y, a, t, (int)(it - turn * parts), parts);
     }
 }
 
-int blocks_for(const nck_dev *d, int64_t want, int per_sm) {
-    const int64_t room = (int64_t)(d->sm_count > 0 ? d->sm_count : 148) * per_sm;
-    return (int)(want < 1 ? 1 : want < room ? want : room);
+// Parts of a row of V logits so that `rows` rows make about `items` parts, none below `least` logits.
+int parts_for(int64_t rows, int64_t V, int64_t items, int64_t least) {
+    int64_t n = (items + rows - 1) / rows;
+    if (n > V / least) n = V / least;
+    return n < 1 ? 1 : (int)n;
+}
+
+// Blocks of a grid-stride launch: one full wave of the kernel, or fewer for less work.
+template <typename K>
+int wave_of(const nck_dev *d, K kernel, int *room) {
+    if (!*room) *room = resident_blocks(d, kernel, 256);
+    return *room;
+}
+
+int at_most(int64_t want, int room) { return (int)(want < 1 ? 1 : want < room ? want : room); }
+
+template <int W, bool ACC>
+void launch_grad(nck_dev *d, const nck_rows *q, const nck_rows_grad *g) {
+    static int room = 0;
+    wave_of(d, k_rows_grad<W, ACC>, &room);
+    const int parts = W == 32 ? 1 : parts_for(q->N, q->V, room, 4096);
+    k_rows_grad<W, ACC><<<at_most((q->N * parts + 256 / W - 1) / (256 / W), 1 << 30), 256, 0, NCK_STREAM(d)>>>(*q, *g, parts);
+    NCK_LAUNCHED(d, 1);
 }
 
 }  // namespace
 
 extern "C" void nck_rows_logp(nck_dev *d, const nck_rows *q, const nck_policy *p) {
+    static int room_warp = 0, room_block = 0, room_parts = 0;
     nck_rows rows = *q;
     rows.status = d->status;
     nck_policy pol;
@@ -348,15 +459,34 @@ extern "C" void nck_rows_logp(nck_dev *d, const nck_rows *q, const nck_policy *p
     else pol = nck_policy{};
     Scope sc(d, "logits_logp", 4.0 * q->N * q->V, 4.0 * q->N * q->V);
     double2 *part = (double2 *)d->scratch;
+    NCK_LAUNCHED(d, 1);
     if (q->V <= kWarpRow) {
-        const int room = (d->sm_count > 0 ? d->sm_count : 148) * 64;  // warps of a full GPU
-        int64_t run = (q->N + room - 1) / room;
+        const int64_t warps = (int64_t)wave_of(d, k_rows_warp, &room_warp) * 8;
+        int64_t run = (q->N + warps - 1) / warps;
         run = run < 1 ? 1 : run > 32 ? 32 : run;
-        k_rows_warp<<<blocks_for(d, (q->N + run * 8 - 1) / (run * 8), 8), 256, 0, NCK_STREAM(d)>>>(rows, pol, (int)run, part,
-                                                                                                d->counters);
-    } else {
-        k_rows_block<<<blocks_for(d, q->N, 8), 256, 0, NCK_STREAM(d)>>>(rows, pol, part, d->counters);
+        k_rows_warp<<<at_most((q->N + run * 8 - 1) / (run * 8), room_warp), 256, 0, NCK_STREAM(d)>>>(rows, pol, (int)run, part,
+                                                                                                 d->counters);
+        return;
     }
+    wave_of(d, k_rows_block, &room_block);
+    // Parts of rows when the SMs would have less than two rows each and rows are long (of 128000 logits: 61 rows 15
+    // instead of 30 us, 122 23 for 31, 244 32 for 36, but 488 52 for 48; of 50001 61 rows 12.3 for 11.9).
+    if (q->N >= 2 * (int64_t)d->sm_count || q->V < 65536) {
+        k_rows_block<<<at_most(q->N, room_block), 256, 0, NCK_STREAM(d)>>>(rows, pol, part, d->counters);
+        return;
+    }
+    wave_of(d, k_rows_parts, &room_parts);
+    const int parts = parts_for(q->N, q->V, (int64_t)room_parts * 8 * 4, 2048);
+    float2 *stats = (float2 *)(part + 4096); // behind the finishing blocks' sums
+    k_rows_parts<<<at_most((q->N * parts + 7) / 8, room_parts), 256, 0, NCK_STREAM(d)>>>(rows, parts, stats);
+    cudaLaunchAttribute early;
+    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    early.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg = {};
+    const int64_t run = (q->N + 4096 * 8 - 1) / (4096 * 8); // (few rows: one)
+    cfg.gridDim = (unsigned)((q->N + run * 8 - 1) / (run * 8)), cfg.blockDim = 256, cfg.stream = NCK_STREAM(d);
+    cfg.attrs = &early, cfg.numAttrs = 1;
+    cudaLaunchKernelEx(&cfg, k_rows_finish, rows, pol, parts, (int)run, (const float2 *)stats, part, d->counters);
     NCK_LAUNCHED(d, 1);
 }
 
@@ -370,13 +500,10 @@ extern "C" void nck_rows_bwd(nck_dev *d, const nck_rows *q, const nck_rows_grad 
     if (q->N == 0) return;
     Scope sc(d, "logits_logp_bwd", 4.0 * q->N * q->V, 8.0 * q->N * q->V);
     if (q->V <= kWarpRow) {
-        const int grid = blocks_for(d, (q->N + 7) / 8, 16);
-        if (g->acc) k_rows_grad<32, true><<<grid, 256, 0, NCK_STREAM(d)>>>(*q, *g);
-        else k_rows_grad<32, false><<<grid, 256, 0, NCK_STREAM(d)>>>(*q, *g);
+        if (g->acc) launch_grad<32, true>(d, q, g);
+        else launch_grad<32, false>(d, q, g);
     } else {
-        const int grid = blocks_for(d, q->N, 16);
-        if (g->acc) k_rows_grad<256, true><<<grid, 256, 0, NCK_STREAM(d)>>>(*q, *g);
-        else k_rows_grad<256, false><<<grid, 256, 0, NCK_STREAM(d)>>>(*q, *g);
+        if (g->acc) launch_grad<256, true>(d, q, g);
+        else launch_grad<256, false>(d, q, g);
     }
-    NCK_LAUNCHED(d, 1);
 }
