@@ -273,12 +273,25 @@ static void plan_release_node(nc_ctx *ctx, nc_node *n, nc_tensor *loss, const bw
 
 nc_status nc_backward(nc_tensor *loss) { return nc_backward_ex(loss, 0, NULL, 0); }
 
-/* d loss / d loss at the start of a pass: 1 stored into a fresh buffer, or added to one that already
- * holds a gradient. With dy (the gradient of y given by the caller), a y that some op produced reads the
- * caller's buffer in place (an alias that owns nothing and is dropped when the pass ends: *lent = 1); a leaf, or a y that holds a gradient already, has dy
- * copied or added into its own. Returns 0 on failure. */
-static int seed_gradient(nc_ctx *ctx, nc_tensor *y, nc_tensor *dy, int *lent) {
+/* d loss / d loss at the start of a pass: 1, or dy (the gradient of y given by the caller). A y that some op
+ * produced and that holds no gradient reads the context's constant 1, or the caller's buffer, in place (an alias
+ * that owns nothing and is dropped when the pass ends: *lent = 1; a retained pass keeps the gradient 1, in a
+ * buffer of its own). Otherwise 1 or dy is stored into a fresh buffer or added to what is there. Returns 0 on
+ * failure. */
+static int seed_gradient(nc_ctx *ctx, nc_tensor *y, nc_tensor *dy, int retain, int *lent) {
     *lent = 0;
+    if (!dy && !retain && y->node && !y->grad) { /* the context's constant 1, the same for every pass */
+        if (!ctx->one) {
+            if (!(ctx->one = nc__tensor_new(ctx, NC_F32, 0, NULL, 1))) return 0;
+            nck_fill_f32(nc__k(ctx), (float *)ctx->one->data, 1.0f, 1);
+        }
+        if (!(y->grad = nc__tensor_alias(ctx->one, 0))) return 0;
+        y->grad->ndim = y->ndim; /* y has one element */
+        memcpy(y->grad->shape, y->shape, sizeof y->shape);
+        nc__contig_strides(y->ndim, y->grad->shape, y->grad->stride);
+        *lent = 1;
+        return 1;
+    }
     if (dy && y->node && !y->grad && nc_is_contiguous(dy)) {
         nc__dev(dy);
         y->grad = nc__tensor_alias(dy, 0);
@@ -367,7 +380,7 @@ static nc_status backward_pass(nc_tensor *loss, nc_tensor *dy, int flags, nc_ten
     }
 
     int lent;
-    if (!seed_gradient(ctx, loss, dy, &lent)) {
+    if (!seed_gradient(ctx, loss, dy, retain, &lent)) {
         plan_free(&pl);
         return ctx->status;
     }

@@ -464,6 +464,7 @@ void nc_free_ctx(nc_ctx *ctx) {
     }
     /* persistent tensor headers are host mallocs owned by their callers' handles; the device
      * blocks were returned above */
+    free(ctx->one);
     free(ctx->pmem);
     nc_hchunk *c = ctx->hchunks;
     while (c) {

@@ -113,16 +113,6 @@ __device__ __forceinline__ Stat warp_join(Stat st) {
     return st;
 }
 
-// lp of a row in 64 bits; the row is read as label 0 (and reported) when its label is out of range
-__device__ __forceinline__ double logp_of(const nck_rows &q, const float *z, int64_t r, Stat st) {
-    int32_t a = q.lab[r];
-    if (a < 0 || a >= q.V) {
-        report(q.status, NCK_ERR_LABEL);
-        a = 0;
-    }
-    return ((double)z[a] - (double)st.m) - log((double)st.s);
-}
-
 __device__ __forceinline__ const float *row_of(const nck_rows &q, int64_t r) {
     const int64_t b = r / q.T;
     return q.z + b * q.sb + (r - b * q.T) * q.st;
@@ -134,16 +124,36 @@ struct Sums {
     double loss, count;
 };
 
+// What a row has besides its statistics: the label's logit and the loss's inputs. The row is read as label 0 (and
+// reported) when its label is out of range.
+struct RowIn {
+    float z, old, ref, adv;
+};
+
+__device__ __forceinline__ RowIn row_in(const nck_rows &q, const nck_policy &p, int64_t r) {
+    int32_t a = q.lab[r];
+    if (a < 0 || a >= q.V) {
+        report(q.status, NCK_ERR_LABEL);
+        a = 0;
+    }
+    RowIn in = {row_of(q, r)[a], 0.0f, 0.0f, 0.0f};
+    if (p.adv) {
+        in.old = p.old[r], in.adv = p.adv[r];
+        if (p.kl != 0.0f) in.ref = p.ref[r];
+    }
+    return in;
+}
+
 // What a row's log probability becomes: its loss term and the factor c of its gradient (without 1 / count).
-__device__ __forceinline__ double policy_term(const nck_policy &p, int64_t r, double lp, float *c) {
-    const float A = p.adv[r], ratio = expf((float)(lp - (double)p.old[r]));
+__device__ __forceinline__ double policy_term(const nck_policy &p, const RowIn &in, double lp, float *c) {
+    const float A = in.adv, ratio = expf((float)(lp - (double)in.old));
     const float lo = 1.0f - p.clip_low, hi = 1.0f + p.clip_high;
     const float held = fminf(fmaxf(ratio, lo), hi);
     const float gain = fminf(ratio * A, held * A);
     const bool moves = A >= 0.0f ? ratio <= hi : ratio >= lo;
     float term = isnan(ratio) ? ratio : -gain, f = moves ? -A * ratio : 0.0f;
     if (p.kl != 0.0f) {
-        const float away = (float)((double)p.ref[r] - lp), e = expm1f(away);
+        const float away = (float)((double)in.ref - lp), e = expm1f(away);
         term += p.kl * (e - away);
         f -= p.kl * e;
     }
@@ -151,14 +161,14 @@ __device__ __forceinline__ double policy_term(const nck_policy &p, int64_t r, do
     return (double)term;
 }
 
-__device__ __forceinline__ Sums finish_row(const nck_rows &q, const nck_policy &p, int64_t r, Stat st) {
-    const double lp = logp_of(q, row_of(q, r), r, st);
+__device__ __forceinline__ Sums finish_row(const nck_rows &q, const nck_policy &p, int64_t r, Stat st, const RowIn &in) {
+    const double lp = ((double)in.z - (double)st.m) - log((double)st.s);
     if (q.stat) reinterpret_cast<float2 *>(q.stat)[r] = make_float2(st.m, 1.0f / st.s);
     if (q.lp64) q.lp64[r] = lp;
     if (q.lp32) q.lp32[r] = (float)lp;
     if (!p.adv) return {0.0, 1.0};
     float c;
-    const double term = policy_term(p, r, lp, &c);
+    const double term = policy_term(p, in, lp, &c);
     if (p.coef) p.coef[r] = c;
     return {term, 1.0};
 }
@@ -218,13 +228,15 @@ __global__ void __launch_bounds__(256) k_rows_warp(nck_rows q, nck_policy p, int
         const bool live = lane < n && counted(q, r0 + lane);
         const unsigned any = __ballot_sync(~0u, live);
         Stat own = {kNone, 0.0f};
+        RowIn in = {};
+        if (live) in = row_in(q, p, r0 + lane); // on its way while the rows are read
         for (int k = 0; k < n; k++) {
             if (!(any >> k & 1)) continue;
             const Stat st = warp_join(read_row<32, 1>(row_of(q, r0 + k), q.V, lane, 0, 1));
             if (lane == k) own = st;
         }
         if (live) {
-            const Sums s = finish_row(q, p, r0 + lane, own);
+            const Sums s = finish_row(q, p, r0 + lane, own, in);
             sums.loss += s.loss, sums.count += s.count;
         } else if (lane < n) {
             skip_row(q, p, r0 + lane);
@@ -239,11 +251,12 @@ __global__ void __launch_bounds__(256) k_rows_block(nck_rows q, nck_policy p, do
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     Sums sums = {0.0, 0.0};
     Stat own = {kNone, 0.0f};
+    RowIn in = {};
     int64_t own_row = -1;
     int turn = 0, held = 0;
     const auto finish = [&]() {
         if (own_row >= 0) {
-            const Sums s = finish_row(q, p, own_row, own);
+            const Sums s = finish_row(q, p, own_row, own, in);
             sums.loss += s.loss, sums.count += s.count;
         }
         own_row = -1, held = 0;
@@ -260,7 +273,7 @@ __global__ void __launch_bounds__(256) k_rows_block(nck_rows q, nck_policy p, do
             Stat all = {kNone, 0.0f};
             if (lane < 8) all = red[turn][lane];
             all = warp_join(all);
-            if (lane == held) own = all, own_row = r;
+            if (lane == held) own = all, own_row = r, in = row_in(q, p, r);
             if (++held == 32) finish();
         }
         turn ^= 1;
@@ -291,6 +304,8 @@ __global__ void __launch_bounds__(256) k_rows_finish(nck_rows q, nck_policy p, i
     const bool live = lane < n && counted(q, r0 + lane);
     const unsigned any = __ballot_sync(~0u, live);
     Stat own = {kNone, 0.0f};
+    RowIn in = {};
+    if (live) in = row_in(q, p, r0 + lane);
     for (int i = 0; i < n; i++) {
         if (!(any >> i & 1)) continue;
         Stat st = {kNone, 0.0f};
@@ -302,7 +317,7 @@ __global__ void __launch_bounds__(256) k_rows_finish(nck_rows q, nck_policy p, i
         if (lane == i) own = st;
     }
     if (live) {
-        const Sums s = finish_row(q, p, r0 + lane, own);
+        const Sums s = finish_row(q, p, r0 + lane, own, in);
         sums.loss += s.loss, sums.count += s.count;
     } else if (lane < n) {
         skip_row(q, p, r0 + lane);

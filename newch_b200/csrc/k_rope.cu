@@ -54,7 +54,7 @@ __device__ __forceinline__ void store(float *p, const float (&v)[VEC]) {
 // How warps share the work: an item is `run` heads (of one weight) of the 32 / LPR tokens of a tile; the items
 // of the query heads come first.
 struct RopeGrid {
-    int run, tiles;          // tiles of tokens
+    int run[2], tiles;       // heads to an item (query, key); tiles of tokens
     int64_t items, q_items;
     FastDiv by_tiles, by_T;
 };
@@ -189,8 +189,9 @@ struct Item {
         const bool query = it < g.q_items;
         const uint32_t k = (uint32_t)(query ? it : it - g.q_items), chunk = g.by_tiles.div(k);
         const int first = query ? 0 : q.HQ, end = query ? q.HQ : q.H;
-        h0 = first + (int)chunk * g.run;
-        h1 = min(h0 + g.run, end);
+        const int run = g.run[query ? 0 : 1];
+        h0 = first + (int)chunk * run;
+        h1 = min(h0 + run, end);
         const int64_t at = (int64_t)(k - chunk * (uint32_t)g.tiles) * per + sub, tokens = q.B * q.T;
         live = sub < per && at < tokens;
         tok = (int)(at < tokens ? at : tokens - 1);
@@ -394,19 +395,23 @@ int vector_of(const nck_rope *q, const void *p1, const void *p2) {
     return 1;
 }
 
-// A run is all heads of a weight when there are tokens enough for several waves of warps, fewer (down to one)
-// when there are not: a shorter run forms the angles more often, a longer one leaves SMs without work.
+// The heads of a weight are one run when the tokens alone fill the GPU's resident warps, and even parts of them
+// (down to single heads) when they do not: a shorter run forms the angles more often, a longer one leaves SMs idle.
 RopeGrid split_of(const nck_dev *d, const nck_rope *q, int lpr) {
     RopeGrid g;
     const int64_t tokens = q->B * q->T, per = 32 / lpr, tiles = (tokens + per - 1) / per;
-    const int64_t want = (int64_t)d->sm_count * 32;
-    int64_t run = tiles * q->H / want;
-    run = run < 1 ? 1 : run > q->H ? q->H : run;
-    const int64_t kh = q->H - q->HQ;
-    g.run = (int)run;
+    const int64_t chunks = (int64_t)d->sm_count * 16 / tiles; // of all heads
+    const int64_t run = chunks < 1 ? q->H : (q->H + chunks - 1) / chunks;
+    const int heads[2] = {q->HQ, q->H - q->HQ};
+    int64_t items[2];
+    for (int k = 0; k < 2; k++) {
+        const int64_t n = (heads[k] + run - 1) / run;
+        g.run[k] = n ? (int)((heads[k] + n - 1) / n) : 1;
+        items[k] = n * tiles;
+    }
     g.tiles = (int)tiles;
-    g.q_items = (q->HQ + run - 1) / run * tiles;
-    g.items = g.q_items + (kh + run - 1) / run * tiles;
+    g.q_items = items[0];
+    g.items = items[0] + items[1];
     g.by_tiles = make_fastdiv((uint32_t)tiles);
     g.by_T = make_fastdiv((uint32_t)q->T);
     return g;

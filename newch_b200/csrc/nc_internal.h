@@ -242,6 +242,7 @@ struct nc_ctx {
 
     /* scratch double accumulators etc. */
     double *dscratch;
+    nc_tensor *one;      /* the gradient 1 that a backward pass starts from (made at first use) */
 };
 
 void *nc__arena_alloc(nc_ctx *ctx, size_t bytes);             /* device, step lifetime */

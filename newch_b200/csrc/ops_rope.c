@@ -86,7 +86,7 @@ static int rope_of(const nc_node *n, nck_rope *q) {
     q->pos_t = q->n_axes;
     q->pos_b = pos && pos->ndim == 3 ? q->T * q->n_axes : 0;
     if (!q->x || (wq && !q->wq) || (wk && !q->wk) || (pos && !q->pos)) return 0;
-    /* turns of pair i per step: base^-(i / half) / 2 pi, by repeated products of 64-bit mantissas (half an
+    /* turns of pair i per step: base^-(i / half) / 2 pi in 2^-64 turns, by repeated products of 64-bit mantissas (half an
      * ulp each), without whole turns; with AXIS_FREQ i counts from the start of its section and half is the
      * section's length */
     const long double unit = 0.159154943091895335768883763372514362L, ln_base = logl((long double)n->p.f[0]);
@@ -95,7 +95,7 @@ static int rope_of(const nc_node *n, nck_rope *q) {
     for (int a = 0, i = 0; a < q->n_axes; a++) {
         const int len = (int)n->p.i[P_SECTION + a];
         if (by_axis && len) f = unit, step = expl(-ln_base / len);
-        for (int j = 0; j < len; j++, i++, f *= step) q->turns[i] = (uint64_t)ldexpl(f - floorl(f), 64), q->axis[i] = (unsigned char)a;
+        for (int j = 0; j < len; j++, i++, f *= step) q->turns[i] = (uint64_t)((f < 1.0L ? f : f - floorl(f)) * 0x1p64L), q->axis[i] = (unsigned char)a;
     }
     return 1;
 }
