@@ -7,14 +7,16 @@
 // 4 bytes a logit forward, 8 backward, about one exponential each, so HBM bounds them. Rows that the mask leaves
 // out are not read; their gradient is zeros.
 //
-// A row of up to kWarpRow logits belongs to a warp, a longer one to a block of 256 threads with many loads in
-// flight a thread (8 vectors forward, 16 backward: 4 x 2048 rows of 50001 logits with half of the rows counted take
-// 123 and 354 us, 0.82 and 2.46 GB at the copy rate 125 and 375; with 4 vectors 128 and 376). A few very long
-// rows are split among warps, and a second launch joins the parts. Statistics of up to 32 rows wait in a warp's lanes,
-// so that the double precision arithmetic of the loss runs once for all of them and not once a row. Backward has a
-// block a row (uncounted rows cost a third, so dealing rows out in advance leaves SMs idle: 418 us) and starts with
-// the last row, whose logits the forward pass may have left in L2. Log probabilities and everything behind them that
-// can cancel (log ratios, sums over tokens and rows) are held in 64 bits; sums run in a fixed order.
+// Many loads in flight are what both need. Rows of up to kSmallRow logits belong to 1 to 32 lanes with several
+// rows of a warp's run in flight (200000 rows of 61 logits, both passes: 63 us; a warp a row took 187); rows of some
+// thousand logits to a warp, the long ones to a block of 256 threads (8 vectors in flight a thread forward, 16
+// backward: 4 x 2048 rows of 50001 logits with half of the rows counted take 123 and 350 us, 0.82 and 2.46 GB at the
+// copy rate 125 and 375; with 4 vectors 128 and 376; 132 forward since its exponential is the exact one). A few very long rows are split among warps, and a second launch
+// joins the parts. Statistics of up to 32 rows wait in a warp's lanes, so that the double precision arithmetic of
+// the loss runs once for all of them and not once a row. Backward deals rows out as blocks end (uncounted rows cost
+// a third, so dealing them out in advance leaves SMs idle: 418 us) and starts with the last long row, whose logits
+// the forward pass may have left in L2. Log probabilities and everything behind them that can cancel (log ratios,
+// sums over tokens and rows) are held in 64 bits; sums run in a fixed order.
 #include <math.h>
 
 #include "k_common.cuh"
@@ -23,15 +25,69 @@ using namespace nck;
 
 namespace {
 
-constexpr int kWarpRow = 1024;
+constexpr int kSmallRow = 512, kShortRow = 1024; // rows read in one go by lanes, by a warp
 constexpr float kNone = -INFINITY;
 
-// e^x by the approximate power of two: off by 2 steps and the rounding of x log2 e; results below 2^-126 are 0
+// e^x of the gradient by the approximate power of two: off by 2 steps and the rounding of x log2 e; results below
+// 2^-126 are 0.
 __device__ __forceinline__ float exp_of(float x) {
     float r;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x * 1.4426950408889634f));
     return r;
 }
+
+// two floats at once (one issue slot for both)
+__device__ __forceinline__ uint64_t two(float x, float y) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+    return r;
+}
+__device__ __forceinline__ uint64_t two(float x) { return two(x, x); }
+__device__ __forceinline__ void apart(uint64_t v, float &x, float &y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+
+__device__ __forceinline__ float at_least(float x, float low) { // NaN stays NaN
+    float y;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(x), "f"(low));
+    return y;
+}
+
+// e^x of the sums, two x <= 0 at once: 2^n times a polynomial in f = x log2 e - n, |f| <= 1/2 (interpolation of
+// (2^f - 1) / f at Chebyshev nodes). It is off by less than 1.5 * 2^-24 and, what matters here, by 7e-10 in the mean:
+// with the approximate power a log probability is 5e-8 to 2e-7 too large in the mean (vocabularies of 96 to 128000),
+// which adds up over the tokens of an answer. x below -87 counts as -87 (2e-38 of the largest term); NaN stays NaN.
+__device__ __forceinline__ uint64_t exp_sum2(uint64_t x) {
+    constexpr float kLog2e = 1.4426950408889634f, kRest = (float)(1.4426950408889634 - (double)kLog2e);
+    constexpr float kRound = 12582912.0f + 127.0f; // adding it rounds to whole numbers; low bits: the number + 127
+    float x0, x1, t0, t1;
+    apart(x, x0, x1);
+    const uint64_t y = two(at_least(x0, -87.0f), at_least(x1, -87.0f));
+    const uint64_t t = fma2(y, two(kLog2e), two(kRound));
+    const uint64_t f = fma2(y, two(kRest), fma2(y, two(kLog2e), fma2(t, two(-1.0f), two(kRound))));
+    uint64_t p = fma2(f, two(0.00015453163f), two(0.0013390863f));
+    p = fma2(p, f, two(0.009618083f));
+    p = fma2(p, f, two(0.05550357f));
+    p = fma2(p, f, two(0.2402265f));
+    p = fma2(p, f, two(0.6931472f));
+    apart(t, t0, t1);
+    return mul2(fma2(p, f, two(1.0f)), two(__uint_as_float(__float_as_uint(t0) << 23), __uint_as_float(__float_as_uint(t1) << 23)));
+}
+
+__device__ __forceinline__ void exp_sum(float x, float y, float &ex, float &ey) { apart(exp_sum2(two(x, y)), ex, ey); }
 
 struct Stat {
     float m, s; // running maximum, and the sum of exp(z - m)
@@ -40,19 +96,31 @@ struct Stat {
 // adds a maximum / sum pair to another; a side without finite values has s = 0
 __device__ __forceinline__ Stat join(Stat a, Stat b) {
     const float m = fmaxf(a.m, b.m), base = m == kNone ? 0.0f : m;
-    return {m, a.s * exp_of(a.m - base) + b.s * exp_of(b.m - base)};
+    float ea, eb;
+    exp_sum(a.m - base, b.m - base, ea, eb);
+    return {m, fmaf(a.s, ea, b.s * eb)};
 }
 
 template <int N>
 __device__ __forceinline__ void take(Stat &st, const float (&v)[N]) {
+    static_assert(N % 2 == 0, "pairs");
     float top = v[0];
 #pragma unroll
     for (int i = 1; i < N; i++) top = fmaxf(top, v[i]);
     const float m = fmaxf(st.m, top), base = m == kNone ? 0.0f : m;
-    float s = st.s * exp_of(st.m - base);
+    const uint64_t down = two(-base);
+    uint64_t sum = exp_sum2(add2(two(v[0], v[1]), down));
 #pragma unroll
-    for (int i = 0; i < N; i++) s += exp_of(v[i] - base);
-    st.m = m, st.s = s;
+    for (int i = 2; i < N; i += 2) sum = add2(sum, exp_sum2(add2(two(v[i], v[i + 1]), down)));
+    if (m != st.m) { // (rarely, once a row's largest values have been met)
+        float e, unused;
+        exp_sum(st.m - base, 0.0f, e, unused);
+        st.s *= e;
+    }
+    float x, y;
+    apart(sum, x, y);
+    st.m = m;
+    st.s += x + y;
 }
 
 // floats before the first 16-byte boundary at or behind p, at most n
@@ -93,12 +161,29 @@ __device__ __forceinline__ Stat read_row(const float *z, int64_t V, int t, int k
     }
     if (k) return st; // part 0 has the ends that are no whole vectors
     const int64_t tail = lead + 4 * (int64_t)nv;
-    if (t < lead) {
-        const float v[1] = {z[t]};
+    if (t < 3) {
+        const float v[2] = {t < lead ? z[t] : kNone, t < V - tail ? z[tail + t] : kNone};
         take(st, v);
     }
-    if (t < V - tail) {
-        const float v[1] = {z[tail + t]};
+    return st;
+}
+
+// A warp reads a row of up to kShortRow logits, all of it in flight at once.
+__device__ __forceinline__ Stat read_short_row(const float *z, int V, int lane) {
+    constexpr int U = kShortRow / 128;
+    const int lead = (int)lead_of(z, V), nv = (V - lead) >> 2, tail = lead + 4 * nv;
+    const float4 *z4 = reinterpret_cast<const float4 *>(z + lead);
+    float4 f[U];
+    const float v0[2] = {lane < lead ? z[lane] : kNone, lane < V - tail ? z[tail + lane] : kNone};
+#pragma unroll
+    for (int u = 0; u < U; u++)
+        f[u] = lane + 32 * u < nv ? __ldg(z4 + lane + 32 * u) : make_float4(kNone, kNone, kNone, kNone);
+    Stat st = {kNone, 0.0f};
+    take(st, v0);
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        if (32 * u >= nv) break;
+        const float v[4] = {f[u].x, f[u].y, f[u].z, f[u].w};
         take(st, v);
     }
     return st;
@@ -114,6 +199,7 @@ __device__ __forceinline__ Stat warp_join(Stat st) {
 }
 
 __device__ __forceinline__ const float *row_of(const nck_rows &q, int64_t r) {
+    if (q.T == q.N) return q.z + r * q.st;
     const int64_t b = r / q.T;
     return q.z + b * q.sb + (r - b * q.T) * q.st;
 }
@@ -232,8 +318,58 @@ __global__ void __launch_bounds__(256) k_rows_warp(nck_rows q, nck_policy p, int
         if (live) in = row_in(q, p, r0 + lane); // on its way while the rows are read
         for (int k = 0; k < n; k++) {
             if (!(any >> k & 1)) continue;
-            const Stat st = warp_join(read_row<32, 1>(row_of(q, r0 + k), q.V, lane, 0, 1));
+            const float *z = row_of(q, r0 + k);
+            const Stat st = warp_join(q.V <= kShortRow ? read_short_row(z, (int)q.V, lane) : read_row<32, 8>(z, q.V, lane, 0, 1));
             if (lane == k) own = st;
+        }
+        if (live) {
+            const Sums s = finish_row(q, p, r0 + lane, own, in);
+            sums.loss += s.loss, sums.count += s.count;
+        } else if (lane < n) {
+            skip_row(q, p, r0 + lane);
+        }
+    }
+    if (p.loss) finish_loss(p, sums, part, counter);
+}
+
+// Rows of up to E G logits: G lanes a row, 32 / G rows a pass and P passes of a warp's run in flight; row i's
+// statistics go to lane i.
+template <int G, int E, int P>
+__global__ void __launch_bounds__(256) k_rows_small(nck_rows q, nck_policy p, int run, double2 *part, unsigned *counter) {
+    constexpr int R = 32 / G;
+    const int lane = threadIdx.x & 31, l = lane % G, V = (int)q.V;
+    const int64_t warps = (int64_t)gridDim.x * 8;
+    Sums sums = {0.0, 0.0};
+    for (int64_t r0 = ((int64_t)blockIdx.x * 8 + (threadIdx.x >> 5)) * run; r0 < q.N; r0 += warps * run) {
+        const int n = q.N - r0 < run ? (int)(q.N - r0) : run;
+        const bool live = lane < n && counted(q, r0 + lane);
+        const unsigned any = __ballot_sync(~0u, live);
+        Stat own = {kNone, 0.0f};
+        RowIn in = {};
+        if (live) in = row_in(q, p, r0 + lane);
+        for (int it = 0; it * R < n; it += P) {
+            float v[P][E];
+#pragma unroll
+            for (int u = 0; u < P; u++) {
+                const int row = (it + u) * R + lane / G;
+                const bool ok = row < n && (any >> row & 1);
+                const float *z = row_of(q, r0 + (ok ? row : 0));
+#pragma unroll
+                for (int e = 0; e < E; e++) v[u][e] = ok && e * G + l < V ? __ldg(z + e * G + l) : kNone;
+            }
+#pragma unroll
+            for (int u = 0; u < P; u++) {
+                Stat st = {kNone, 0.0f};
+                take(st, v[u]);
+#pragma unroll
+                for (int o = G / 2; o > 0; o >>= 1) {
+                    const Stat b = {__shfl_xor_sync(~0u, st.m, o), __shfl_xor_sync(~0u, st.s, o)};
+                    st = join(st, b);
+                }
+                const int from = lane % R * G;
+                const Stat mine = {__shfl_sync(~0u, st.m, from), __shfl_sync(~0u, st.s, from)};
+                if (lane / R == it + u) own = mine;
+            }
         }
         if (live) {
             const Sums s = finish_row(q, p, r0 + lane, own, in);
@@ -434,7 +570,62 @@ __global__ void __launch_bounds__(256) k_rows_grad(nck_rows q, nck_rows_grad g, 
         const float2 st = c == 0.0f ? make_float2(0.f, 0.f) : reinterpret_cast<const float2 *>(q.stat)[r];
         int64_t a = q.lab[r];
         if (a < 0 || a >= q.V) a = 0;
-        grad_row<W, W == 32 ? 1 : ACC ? 8 : 16, ACC>(row_of(q, r), g.dz + r * q.V, q.V, c, st.x, st.y, a, t, (int)(it - turn * parts), parts);
+        grad_row<W, W == 32 || ACC ? 8 : 16, ACC>(row_of(q, r), g.dz + r * q.V, q.V, c, st.x, st.y, a, t, (int)(it - turn * parts), parts);
+    }
+}
+
+// The gradient of rows of up to E G logits, G lanes a row: a warp takes a run of rows, lane i fetching what row i needs.
+template <int G, int E, int P, bool ACC>
+__global__ void __launch_bounds__(256) k_rows_grad_small(nck_rows q, nck_rows_grad g, int run) {
+    constexpr int R = 32 / G;
+    const int lane = threadIdx.x & 31, l = lane % G, V = (int)q.V;
+    const float up = g.up[0] * (g.scale ? g.scale[0] : 1.0f);
+    const int64_t r0 = ((int64_t)blockIdx.x * 8 + (threadIdx.x >> 5)) * run;
+    if (r0 >= q.N) return;
+    const int n = q.N - r0 < run ? (int)(q.N - r0) : run;
+    float c = 0.0f;
+    float2 st = make_float2(0.0f, 0.0f);
+    int a = 0;
+    if (lane < n) {
+        const int64_t r = r0 + lane;
+        if (counted(q, r)) c = up * g.coef[r / g.per_coef];
+        if (c != 0.0f) {
+            st = reinterpret_cast<const float2 *>(q.stat)[r];
+            a = q.lab[r];
+            if (a < 0 || a >= V) a = 0;
+        }
+    }
+    for (int it = 0; it * R < n; it += P) {
+        float v[P][E], old[ACC ? P : 1][ACC ? E : 1];
+#pragma unroll
+        for (int u = 0; u < P; u++) {
+            const int row = (it + u) * R + lane / G;
+            const float rc = __shfl_sync(~0u, c, row & 31);
+            const bool ok = row < n, read = ok && rc != 0.0f;
+            const float *z = row_of(q, r0 + (ok ? row : 0));
+            const float *dz = g.dz + (r0 + (ok ? row : 0)) * V;
+#pragma unroll
+            for (int e = 0; e < E; e++) {
+                v[u][e] = read && e * G + l < V ? __ldg(z + e * G + l) : kNone;
+                if (ACC) old[ACC ? u : 0][ACC ? e : 0] = read && e * G + l < V ? dz[e * G + l] : 0.0f;
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < P; u++) {
+            const int row = (it + u) * R + lane / G, s = row & 31;
+            const float rc = __shfl_sync(~0u, c, s), m = __shfl_sync(~0u, st.x, s), inv = __shfl_sync(~0u, st.y, s);
+            const int ra = __shfl_sync(~0u, a, s);
+            if (row >= n || (ACC && rc == 0.0f)) continue;
+            float *dz = g.dz + (r0 + row) * V;
+#pragma unroll
+            for (int e = 0; e < E; e++) {
+                const int j = e * G + l;
+                if (j >= V) break;
+                float d = rc == 0.0f ? 0.0f : -rc * inv * exp_of(v[u][e] - m);
+                if (j == ra) d += rc;
+                dz[j] = ACC ? old[ACC ? u : 0][ACC ? e : 0] + d : d;
+            }
+        }
     }
 }
 
@@ -463,6 +654,42 @@ void launch_grad(nck_dev *d, const nck_rows *q, const nck_rows_grad *g) {
     NCK_LAUNCHED(d, 1);
 }
 
+// Whether a row belongs to a warp and not to a block: short rows, and middling ones when there are enough of them
+// to fill the GPU with warps. Both passes, warp and block: 50000 rows of 1500 logits 177 and 745 us, 500 rows 14.6
+// and 17.6; 2000 rows of 8000 46 and 56 us, 500 rows 31 and 23; 8192 rows of 16000 281 and 273.
+bool warp_rows(const nck_rows *q) { return q->V <= 2048 || (q->V <= 12288 && q->N >= 1024); }
+
+// Rows to a warp: as few as fill the resident warps, at most 32.
+int run_for(const nck_dev *d, int64_t rows, int room) {
+    const int64_t run = (rows + (int64_t)room * 8 - 1) / ((int64_t)room * 8);
+    return (int)(run < 1 ? 1 : run > 32 ? 32 : run);
+}
+
+template <int G, int E, int P>
+void launch_small(nck_dev *d, const nck_rows *q, const nck_policy *p, const nck_rows_grad *g) {
+    static int room = 0;
+    wave_of(d, k_rows_small<G, E, P>, &room);
+    constexpr int R = 32 / G;
+    const int run = (run_for(d, q->N, room) + R - 1) / R * R; // whole passes
+    const int64_t blocks = (q->N + run * 8 - 1) / (run * 8);
+    if (p) k_rows_small<G, E, P><<<at_most(blocks, room), 256, 0, NCK_STREAM(d)>>>(*q, *p, run, (double2 *)d->scratch, d->counters);
+    else if (g->acc) k_rows_grad_small<G, E, P, true><<<(unsigned)blocks, 256, 0, NCK_STREAM(d)>>>(*q, *g, run);
+    else k_rows_grad_small<G, E, P, false><<<(unsigned)blocks, 256, 0, NCK_STREAM(d)>>>(*q, *g, run);
+    NCK_LAUNCHED(d, 1);
+}
+
+// Rows of up to kSmallRow logits, forward (p) or backward (g).
+void dispatch_small(nck_dev *d, const nck_rows *q, const nck_policy *p, const nck_rows_grad *g) {
+    if (q->V <= 4) launch_small<1, 4, 4>(d, q, p, g);
+    else if (q->V <= 8) launch_small<2, 4, 4>(d, q, p, g);
+    else if (q->V <= 16) launch_small<4, 4, 4>(d, q, p, g);
+    else if (q->V <= 32) launch_small<8, 4, 4>(d, q, p, g);
+    else if (q->V <= 64) launch_small<16, 4, 4>(d, q, p, g);
+    else if (q->V <= 128) launch_small<32, 4, 4>(d, q, p, g);
+    else if (q->V <= 256) launch_small<32, 8, 4>(d, q, p, g);
+    else launch_small<32, 16, 2>(d, q, p, g);
+}
+
 }  // namespace
 
 extern "C" void nck_rows_logp(nck_dev *d, const nck_rows *q, const nck_policy *p) {
@@ -474,11 +701,13 @@ extern "C" void nck_rows_logp(nck_dev *d, const nck_rows *q, const nck_policy *p
     else pol = nck_policy{};
     Scope sc(d, "logits_logp", 4.0 * q->N * q->V, 4.0 * q->N * q->V);
     double2 *part = (double2 *)d->scratch;
+    if (q->V <= kSmallRow) {
+        dispatch_small(d, &rows, &pol, nullptr);
+        return;
+    }
     NCK_LAUNCHED(d, 1);
-    if (q->V <= kWarpRow) {
-        const int64_t warps = (int64_t)wave_of(d, k_rows_warp, &room_warp) * 8;
-        int64_t run = (q->N + warps - 1) / warps;
-        run = run < 1 ? 1 : run > 32 ? 32 : run;
+    if (warp_rows(q)) {
+        const int64_t run = run_for(d, q->N, wave_of(d, k_rows_warp, &room_warp));
         k_rows_warp<<<at_most((q->N + run * 8 - 1) / (run * 8), room_warp), 256, 0, NCK_STREAM(d)>>>(rows, pol, (int)run, part,
                                                                                                  d->counters);
         return;
@@ -514,7 +743,9 @@ extern "C" void nck_pref_pairs(nck_dev *d, const nck_pairs *p, const double *lp)
 extern "C" void nck_rows_bwd(nck_dev *d, const nck_rows *q, const nck_rows_grad *g) {
     if (q->N == 0) return;
     Scope sc(d, "logits_logp_bwd", 4.0 * q->N * q->V, 8.0 * q->N * q->V);
-    if (q->V <= kWarpRow) {
+    if (q->V <= kSmallRow) {
+        dispatch_small(d, q, nullptr, g);
+    } else if (warp_rows(q)) {
         if (g->acc) launch_grad<32, true>(d, q, g);
         else launch_grad<32, false>(d, q, g);
     } else {
