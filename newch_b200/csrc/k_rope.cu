@@ -13,7 +13,7 @@
 // multiplies them by the weights once, and keeps them in registers: no table in memory, no barrier. Warps walk
 // a grid of one full wave. A group need not be a power of two of lanes: three heads of 72 or 80 share a
 // warp on nine or ten lanes each, where two on sixteen would leave half the issue slots idle (24 x 1369 x 24 heads
-// of 72: 88 instead of 102 us).
+// of 72: 88 instead of 102 us; 4 x 8000 x 16 heads of 66 69 instead of 131).
 //
 // Angles are formed in whole numbers: a pair's turns per step are kept as a 64-bit fraction of a turn, a
 // position times it modulo 2^64 is the fraction of the turn reached, exact to 2^-34 turns at any i32 position,
@@ -51,21 +51,22 @@ __device__ __forceinline__ void store(float *p, const float (&v)[VEC]) {
     else *reinterpret_cast<float4 *>(p) = make_float4(v[0], v[1], v[2], v[3]);
 }
 
-// How warps share the work: an item is `run` heads (of one weight) of the 32 / LPR tokens of a tile; the items
-// of the query heads come first.
+// How warps share the work: an item is `run` heads of the 32 / LPR tokens of a tile.
 struct RopeGrid {
-    int run[2], tiles;       // heads to an item (query, key); tiles of tokens
-    int64_t items, q_items;
+    int run, tiles;          // tiles of tokens
+    int64_t items;
     FastDiv by_tiles, by_T;
 };
 
 constexpr int kOwn = 4, kTwo = kOwn / 2; // pairs per lane, and their register pairs
 
-// Rows that a lane has in flight, two blocks of 256 threads an SM (128 registers a thread). More blocks of fewer
-// rows keep less in flight for the same registers: forward at 4 x 4680 x 24 heads of 128 takes 81 us with 2
-// blocks of 6 rows (70 at the copy rate), 82 with 3 of 2, 84 with 4 of 2; at 24 x 1369 x 24 heads of 72 82, 89 and
-// 88 us (69 at the copy rate). Backward at the first takes 118 us with 2 of 2 (105 at the copy rate), 132 with 3 of 1, 130 with 2 of 3.
-constexpr int kRowsFwd = 6, kRowsBwd = 2;
+// Rows that a lane has in flight, two blocks of 256 threads an SM (128 registers a thread); narrower vectors have more
+// addresses a row and take a row less. More blocks of fewer rows keep less in flight for the same registers. Forward at
+// 4 x 4680 x 24 heads of 128: 78 us with 4 rows (70 at the copy rate), 79 with 3, 80.5 with 6, 85 with 8, and 82 to 84
+// with 3 or 4 blocks of 2; 24 x 1369 x 24 heads of 72: 89, 95, 84, 85 and 88 us (69 at the copy rate); 4 x 8000 x 16
+// heads of 64 50, 53, 51 and 52 us (41). Backward at the first: 118 us with 2 rows (105 at the copy rate), 132 with
+// 3 blocks of 1, 130 with 3 rows.
+constexpr int kRowsFwd = 4, kRowsBwd = 2;
 
 // The pairs of one row that a lane owns, kOwn / VEC vectors of VEC pairs: the first and the second elements of
 // each pair. Pairs behind the row's end read as zero.
@@ -186,12 +187,9 @@ struct Item {
     bool live;
     __device__ __forceinline__ Item(const nck_rope &q, const RopeGrid &g, int64_t it, int sub) {
         constexpr int per = 32 / LPR;
-        const bool query = it < g.q_items;
-        const uint32_t k = (uint32_t)(query ? it : it - g.q_items), chunk = g.by_tiles.div(k);
-        const int first = query ? 0 : q.HQ, end = query ? q.HQ : q.H;
-        const int run = g.run[query ? 0 : 1];
-        h0 = first + (int)chunk * run;
-        h1 = min(h0 + run, end);
+        const uint32_t k = (uint32_t)it, chunk = g.by_tiles.div(k);
+        h0 = (int)chunk * g.run;
+        h1 = min(h0 + g.run, q.H);
         const int64_t at = (int64_t)(k - chunk * (uint32_t)g.tiles) * per + sub, tokens = q.B * q.T;
         live = sub < per && at < tokens;
         tok = (int)(at < tokens ? at : tokens - 1);
@@ -202,7 +200,7 @@ struct Item {
 
 template <int VEC, int LPR, bool INTER>
 __global__ void __launch_bounds__(256, 2) k_rope_fwd(const __grid_constant__ nck_rope q, const RopeGrid g, float *__restrict__ y) {
-    constexpr int U = VEC == 4 ? kRowsFwd : kRowsFwd / 2; // (more addresses a row: fewer rows without spills)
+    constexpr int U = VEC == 4 ? kRowsFwd : kRowsFwd - 1;
     typedef Own<VEC, LPR, INTER> Row;
     const int lane = threadIdx.x & 31, l = lane % LPR, half = q.D >> 1;
     const float inv_d = 1.0f / (float)q.D;
@@ -216,18 +214,21 @@ __global__ void __launch_bounds__(256, 2) k_rope_fwd(const __grid_constant__ nck
 #pragma unroll
         for (int k = 0; k < U; k++)
             if (m.h0 + k < m.h1) row[k].get(x + k * q.sh, half, l);
-        // y_a = r (x_a ac - x_b bs), y_b = r (x_b bc + x_a as)
+        float2 c[kTwo], s[kTwo];
+        turns.template at<VEC, LPR>(q, m.b, m.t, l, c, s);
+        // y_a = r (x_a ac - x_b bs), y_b = r (x_b bc + x_a as), from the weight of the heads that follow
         float2 ac[kTwo], as[kTwo], bc[kTwo], bs[kTwo];
-        turns.template at<VEC, LPR>(q, m.b, m.t, l, ac, as);
-        const float *w = m.h0 < q.HQ ? q.wq : q.wk;
-        Row ws;
-        if (w) ws.get(w, half, l);
-        else ws.fill(1.0f);
+        const auto weigh = [&](const float *w) {
+            Row ws;
+            if (w) ws.get(w, half, l);
+            else ws.fill(1.0f);
 #pragma unroll
-        for (int i = 0; i < kTwo; i++) {
-            bc[i] = mul2(ac[i], ws.b[i]), bs[i] = neg2(mul2(as[i], ws.b[i]));
-            ac[i] = mul2(ac[i], ws.a[i]), as[i] = mul2(as[i], ws.a[i]);
-        }
+            for (int i = 0; i < kTwo; i++) {
+                bc[i] = mul2(c[i], ws.b[i]), bs[i] = neg2(mul2(s[i], ws.b[i]));
+                ac[i] = mul2(c[i], ws.a[i]), as[i] = mul2(s[i], ws.a[i]);
+            }
+        };
+        weigh(m.h0 < q.HQ ? q.wq : q.wk);
         const auto turn = [&](Row &v, float *to) {
             float r = 1.0f;
             if (q.norm) {
@@ -247,8 +248,11 @@ __global__ void __launch_bounds__(256, 2) k_rope_fwd(const __grid_constant__ nck
         };
         for (int h = m.h0;;) {
 #pragma unroll
-            for (int k = 0; k < U; k++)
-                if (h + k < m.h1) turn(row[k], out + k * q.D);
+            for (int k = 0; k < U; k++) {
+                if (h + k >= m.h1) break;
+                if (h + k == q.HQ && h + k > m.h0) weigh(q.wk); // the key heads begin within the run
+                turn(row[k], out + k * q.D);
+            }
             h += U, x += U * q.sh, out += U * q.D;
             if (h >= m.h1) break;
 #pragma unroll
@@ -263,85 +267,89 @@ template <int VEC, int LPR, bool INTER>
 __global__ void __launch_bounds__(256, 2) k_rope_bwd(const __grid_constant__ nck_rope q, const RopeGrid g,
                                                   const float *__restrict__ dy, float *dx, int acc,
                                                   float *__restrict__ part) {
-    constexpr int kPer = 32 / LPR, kGroups = 8 * kPer, U = VEC == 1 ? 1 : kRowsBwd;
+    constexpr int kPer = 32 / LPR, kGroups = 8 * kPer, U = VEC == 4 ? kRowsBwd : kRowsBwd - 1;
     typedef Own<VEC, LPR, INTER> Row;
     __shared__ float red[kGroups * 2 * LPR * kOwn];
     const int lane = threadIdx.x & 31, l = lane % LPR, half = q.D >> 1;
     const float inv_d = 1.0f / (float)q.D;
     __shared__ Turns turns;
     turns.fill(q);
-    const int64_t step = (int64_t)gridDim.x * 8;
-    int64_t it = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-#pragma unroll 1
-    for (int side = 0; side < 2; side++) { // query heads, then key heads
-        const float *w = side ? q.wk : q.wq;
-        Row ws, sum;
-        if (w) ws.get(w, half, l);
-        else ws.fill(1.0f);
-        sum.fill(0.0f);
-        for (const int64_t end = side ? g.items : g.q_items; it < end; it += step) {
-            const Item<LPR> m(q, g, it, lane / LPR);
-            const float *x = q.x + m.b * q.sb + m.t * q.st + m.h0 * q.sh;
-            const int64_t at = ((int64_t)m.tok * q.H + m.h0) * q.D;
-            const float *from = dy + at;
-            float *to = dx + at;
-            Row x_row[U], dy_row[U]; // the first rows are on their way while the angles are formed
-            const auto fetch = [&](int h) {
+    Row sum[2]; // of query heads, of key heads
+    sum[0].fill(0.0f), sum[1].fill(0.0f);
+    for (int64_t it = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); it < g.items; it += (int64_t)gridDim.x * 8) {
+        const Item<LPR> m(q, g, it, lane / LPR);
+        const float *x = q.x + m.b * q.sb + m.t * q.st + m.h0 * q.sh;
+        const int64_t at = ((int64_t)m.tok * q.H + m.h0) * q.D;
+        const float *from = dy + at;
+        float *to = dx + at;
+        Row x_row[U], dy_row[U]; // the first rows are on their way while the angles are formed
+        const auto fetch = [&](int h) {
 #pragma unroll
-                for (int k = 0; k < U; k++)
-                    if (h + k < m.h1) x_row[k].get(x + k * q.sh, half, l), dy_row[k].get(from + k * q.D, half, l);
-            };
-            fetch(m.h0);
-            float2 c[kTwo], s[kTwo];
-            turns.template at<VEC, LPR>(q, m.b, m.t, l, c, s);
-            const auto turn_back = [&](Row &v, Row &d, float *to) {
-                float2 ss = both(0.0f), dot = both(0.0f);
+            for (int k = 0; k < U; k++)
+                if (h + k < m.h1) x_row[k].get(x + k * q.sh, half, l), dy_row[k].get(from + k * q.D, half, l);
+        };
+        fetch(m.h0);
+        float2 c[kTwo], s[kTwo];
+        turns.template at<VEC, LPR>(q, m.b, m.t, l, c, s);
+        Row ws;
+        const auto weigh = [&](const float *w) {
+            if (w) ws.get(w, half, l);
+            else ws.fill(1.0f);
+        };
+        weigh(m.h0 < q.HQ ? q.wq : q.wk);
+        const auto turn_back = [&](Row &v, Row &d, float *to, Row &part_sum) {
+            float2 ss = both(0.0f), dot = both(0.0f);
 #pragma unroll
-                for (int i = 0; i < kTwo; i++) {
-                    const float2 ya = d.a[i], yb = d.b[i];
-                    d.a[i] = fma2(ya, c[i], mul2(yb, s[i]));
-                    d.b[i] = fma2(yb, c[i], neg2(mul2(ya, s[i])));
-                    ss = fma2(v.a[i], v.a[i], fma2(v.b[i], v.b[i], ss));
-                    dot = fma2(mul2(d.a[i], ws.a[i]), v.a[i], fma2(mul2(d.b[i], ws.b[i]), v.b[i], dot));
-                }
-                float r = 1.0f, k = 0.0f; // dx = r g w + k x, k = -r^3 sum(g w x) / D
-                if (q.norm) {
-                    const float all = group_sum<LPR>(sum2(ss), lane, l), mean = group_sum<LPR>(sum2(dot), lane, l) * inv_d;
-                    r = rsqrtf(fmaf(all, inv_d, q.eps));
-                    k = -(mean * r) * (r * r);
-                }
-                if (!m.live) return;
-                Row o;
-#pragma unroll
-                for (int i = 0; i < kTwo; i++) {
-                    const float2 ga = mul2(d.a[i], both(r)), gb = mul2(d.b[i], both(r));
-                    sum.a[i] = fma2(ga, v.a[i], sum.a[i]);
-                    sum.b[i] = fma2(gb, v.b[i], sum.b[i]);
-                    o.a[i] = fma2(ga, ws.a[i], mul2(both(k), v.a[i]));
-                    o.b[i] = fma2(gb, ws.b[i], mul2(both(k), v.b[i]));
-                }
-                if (dx && acc) { // added to what is there
-                    v.get(to, half, l);
-#pragma unroll
-                    for (int i = 0; i < kTwo; i++) {
-                        o.a[i] = fma2(v.a[i], both(1.0f), o.a[i]);
-                        o.b[i] = fma2(v.b[i], both(1.0f), o.b[i]);
-                    }
-                }
-                if (dx) o.put(to, half, l);
-            };
-            for (int h = m.h0;;) {
-#pragma unroll
-                for (int k = 0; k < U; k++)
-                    if (h + k < m.h1) turn_back(x_row[k], dy_row[k], to + k * q.D);
-                h += U, x += U * q.sh, from += U * q.D, to += U * q.D;
-                if (h >= m.h1) break;
-                fetch(h);
+            for (int i = 0; i < kTwo; i++) {
+                const float2 ya = d.a[i], yb = d.b[i];
+                d.a[i] = fma2(ya, c[i], mul2(yb, s[i]));
+                d.b[i] = fma2(yb, c[i], neg2(mul2(ya, s[i])));
+                ss = fma2(v.a[i], v.a[i], fma2(v.b[i], v.b[i], ss));
+                dot = fma2(mul2(d.a[i], ws.a[i]), v.a[i], fma2(mul2(d.b[i], ws.b[i]), v.b[i], dot));
             }
+            float r = 1.0f, k = 0.0f; // dx = r g w + k x, k = -r^3 sum(g w x) / D
+            if (q.norm) {
+                const float all = group_sum<LPR>(sum2(ss), lane, l), mean = group_sum<LPR>(sum2(dot), lane, l) * inv_d;
+                r = rsqrtf(fmaf(all, inv_d, q.eps));
+                k = -(mean * r) * (r * r);
+            }
+            if (!m.live) return;
+            Row o;
+#pragma unroll
+            for (int i = 0; i < kTwo; i++) {
+                const float2 ga = mul2(d.a[i], both(r)), gb = mul2(d.b[i], both(r));
+                part_sum.a[i] = fma2(ga, v.a[i], part_sum.a[i]);
+                part_sum.b[i] = fma2(gb, v.b[i], part_sum.b[i]);
+                o.a[i] = fma2(ga, ws.a[i], mul2(both(k), v.a[i]));
+                o.b[i] = fma2(gb, ws.b[i], mul2(both(k), v.b[i]));
+            }
+            if (dx && acc) { // added to what is there
+                v.get(to, half, l);
+#pragma unroll
+                for (int i = 0; i < kTwo; i++) {
+                    o.a[i] = fma2(v.a[i], both(1.0f), o.a[i]);
+                    o.b[i] = fma2(v.b[i], both(1.0f), o.b[i]);
+                }
+            }
+            if (dx) o.put(to, half, l);
+        };
+        for (int h = m.h0;;) {
+#pragma unroll
+            for (int k = 0; k < U; k++) {
+                if (h + k >= m.h1) break;
+                if (h + k == q.HQ && h + k > m.h0) weigh(q.wk); // the key heads begin within the run
+                if (h + k < q.HQ) turn_back(x_row[k], dy_row[k], to + k * q.D, sum[0]);
+                else turn_back(x_row[k], dy_row[k], to + k * q.D, sum[1]);
+            }
+            h += U, x += U * q.sh, from += U * q.D, to += U * q.D;
+            if (h >= m.h1) break;
+            fetch(h);
         }
-        if (!part) continue;
+    }
+    if (!part) return;
+    for (int side = 0; side < 2; side++) {
         __syncthreads();
-        if (lane < kPer * LPR) sum.put(red + ((threadIdx.x >> 5) * kPer + lane / LPR) * q.D, half, l);
+        if (lane < kPer * LPR) sum[side].put(red + ((threadIdx.x >> 5) * kPer + lane / LPR) * q.D, half, l);
         __syncthreads();
         for (int d = threadIdx.x; d < q.D; d += blockDim.x) {
             float t = 0.0f;
@@ -395,23 +403,16 @@ int vector_of(const nck_rope *q, const void *p1, const void *p2) {
     return 1;
 }
 
-// The heads of a weight are one run when the tokens alone fill the GPU's resident warps, and even parts of them
-// (down to single heads) when they do not: a shorter run forms the angles more often, a longer one leaves SMs idle.
+// All heads are one run when the tokens alone fill the GPU's resident warps, and even parts of them (down to single
+// heads) when they do not: a shorter run forms the angles more often, a longer one leaves SMs idle.
 RopeGrid split_of(const nck_dev *d, const nck_rope *q, int lpr) {
     RopeGrid g;
     const int64_t tokens = q->B * q->T, per = 32 / lpr, tiles = (tokens + per - 1) / per;
-    const int64_t chunks = (int64_t)d->sm_count * 16 / tiles; // of all heads
-    const int64_t run = chunks < 1 ? q->H : (q->H + chunks - 1) / chunks;
-    const int heads[2] = {q->HQ, q->H - q->HQ};
-    int64_t items[2];
-    for (int k = 0; k < 2; k++) {
-        const int64_t n = (heads[k] + run - 1) / run;
-        g.run[k] = n ? (int)((heads[k] + n - 1) / n) : 1;
-        items[k] = n * tiles;
-    }
+    int64_t chunks = (int64_t)d->sm_count * 16 / tiles;
+    chunks = chunks < 1 ? 1 : chunks > q->H ? q->H : chunks;
+    g.run = (int)((q->H + chunks - 1) / chunks);
     g.tiles = (int)tiles;
-    g.q_items = items[0];
-    g.items = items[0] + items[1];
+    g.items = (q->H + g.run - 1) / g.run * tiles;
     g.by_tiles = make_fastdiv((uint32_t)tiles);
     g.by_T = make_fastdiv((uint32_t)q->T);
     return g;
@@ -433,25 +434,29 @@ int launch(nck_dev *d, const nck_rope *q, float *y, const float *dy, float *dx, 
     return grid;
 }
 
-// Vectors of four pairs on as many lanes as a row has vectors, up to the number that lets as many rows share a
-// warp; rows that only narrower vectors fit take a whole warp each.
+// As many lanes as a row needs at four pairs a lane, up to the number that lets as many rows share a warp.
+template <int VEC, bool INTER>
+int by_lanes(nck_dev *d, const nck_rope *q, float *y, const float *dy, float *dx, int acc, float *part) {
+    switch (32 / ((q->D / 2 + kOwn - 1) / kOwn)) { // rows to a warp
+    case 32: return launch<VEC, 1, INTER>(d, q, y, dy, dx, acc, part);
+    case 16: return launch<VEC, 2, INTER>(d, q, y, dy, dx, acc, part);
+    case 10: return launch<VEC, 3, INTER>(d, q, y, dy, dx, acc, part);
+    case 8: return launch<VEC, 4, INTER>(d, q, y, dy, dx, acc, part);
+    case 6: return launch<VEC, 5, INTER>(d, q, y, dy, dx, acc, part);
+    case 5: return launch<VEC, 6, INTER>(d, q, y, dy, dx, acc, part);
+    case 4: return launch<VEC, 8, INTER>(d, q, y, dy, dx, acc, part);
+    case 3: return launch<VEC, 10, INTER>(d, q, y, dy, dx, acc, part);
+    case 2: return launch<VEC, 16, INTER>(d, q, y, dy, dx, acc, part);
+    default: return launch<VEC, 32, INTER>(d, q, y, dy, dx, acc, part);
+    }
+}
+
 template <bool INTER>
 int dispatch(nck_dev *d, const nck_rope *q, float *y, const float *dy, float *dx, int acc, float *part) {
     const int vec = y ? vector_of(q, y, nullptr) : vector_of(q, dy, dx);
-    if (vec == 1) return launch<1, 32, INTER>(d, q, y, dy, dx, acc, part);
-    if (vec == 2) return launch<2, 32, INTER>(d, q, y, dy, dx, acc, part);
-    switch (32 / (q->D / 8)) { // rows to a warp
-    case 32: return launch<4, 1, INTER>(d, q, y, dy, dx, acc, part);
-    case 16: return launch<4, 2, INTER>(d, q, y, dy, dx, acc, part);
-    case 10: return launch<4, 3, INTER>(d, q, y, dy, dx, acc, part);
-    case 8: return launch<4, 4, INTER>(d, q, y, dy, dx, acc, part);
-    case 6: return launch<4, 5, INTER>(d, q, y, dy, dx, acc, part);
-    case 5: return launch<4, 6, INTER>(d, q, y, dy, dx, acc, part);
-    case 4: return launch<4, 8, INTER>(d, q, y, dy, dx, acc, part);
-    case 3: return launch<4, 10, INTER>(d, q, y, dy, dx, acc, part);
-    case 2: return launch<4, 16, INTER>(d, q, y, dy, dx, acc, part);
-    default: return launch<4, 32, INTER>(d, q, y, dy, dx, acc, part);
-    }
+    if (vec == 1) return by_lanes<1, INTER>(d, q, y, dy, dx, acc, part);
+    if (vec == 2) return by_lanes<2, INTER>(d, q, y, dy, dx, acc, part);
+    return by_lanes<4, INTER>(d, q, y, dy, dx, acc, part);
 }
 
 }  // namespace
