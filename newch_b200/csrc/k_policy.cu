@@ -715,7 +715,7 @@ extern "C" void nck_rows_logp(nck_dev *d, const nck_rows *q, const nck_policy *p
     wave_of(d, k_rows_block, &room_block);
     // Parts of rows when the SMs would have less than two rows each and rows are long (of 128000 logits: 61 rows 15
     // instead of 30 us, 122 23 for 31, 244 32 for 36, but 488 52 for 48; of 50001 61 rows 12.3 for 11.9).
-    if (q->N >= 2 * (int64_t)d->sm_count || q->V < 65536) {
+    if (q->N >= 2 * (int64_t)d->sm_count || q->V < 65536 || q->N == 0) {
         k_rows_block<<<at_most(q->N, room_block), 256, 0, NCK_STREAM(d)>>>(rows, pol, part, d->counters);
         return;
     }
