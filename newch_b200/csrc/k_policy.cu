@@ -8,7 +8,7 @@
 // out are not read; their gradient is zeros.
 //
 // Many loads in flight are what both need. Rows of up to kSmallRow logits belong to 1 to 32 lanes with several
-// rows of a warp's run in flight (200000 rows of 61 logits, both passes: 63 us; a warp a row took 187); rows of some
+// rows of a warp's run in flight (200000 rows of 61 logits, both passes: 51 us; a warp a row took 187); rows of some
 // thousand logits to a warp, the long ones to a block of 256 threads (8 vectors in flight a thread forward, 16
 // backward: 4 x 2048 rows of 50001 logits with half of the rows counted take 123 and 350 us, 0.82 and 2.46 GB at the
 // copy rate 125 and 375; with 4 vectors 128 and 376; 132 forward since its exponential is the exact one). A few very long rows are split among warps, and a second launch
@@ -189,13 +189,39 @@ __device__ __forceinline__ Stat read_short_row(const float *z, int V, int lane) 
     return st;
 }
 
+// The statistics of W neighbouring lanes together, in all of them: the maximum first, so each sum is brought to it once.
+template <int W = 32>
 __device__ __forceinline__ Stat warp_join(Stat st) {
+    float m = st.m;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        const Stat b = {__shfl_xor_sync(~0u, st.m, o), __shfl_xor_sync(~0u, st.s, o)};
-        st = join(st, b);
-    }
-    return st;
+    for (int o = W / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
+    float e, unused;
+    exp_sum(st.m - (m == kNone ? 0.0f : m), 0.0f, e, unused);
+    float s = st.s * e;
+#pragma unroll
+    for (int o = W / 2; o > 0; o >>= 1) s += __shfl_xor_sync(~0u, s, o);
+    return {m, s};
+}
+
+// The statistics of the values that W neighbouring lanes hold, in all of them.
+template <int W, int N>
+__device__ __forceinline__ Stat lanes_stat(const float (&v)[N]) {
+    static_assert(N % 2 == 0, "pairs");
+    float m = v[0];
+#pragma unroll
+    for (int i = 1; i < N; i++) m = fmaxf(m, v[i]);
+#pragma unroll
+    for (int o = W / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
+    const uint64_t down = two(m == kNone ? 0.0f : -m);
+    uint64_t sum = exp_sum2(add2(two(v[0], v[1]), down));
+#pragma unroll
+    for (int i = 2; i < N; i += 2) sum = add2(sum, exp_sum2(add2(two(v[i], v[i + 1]), down)));
+    float x, y;
+    apart(sum, x, y);
+    float s = x + y;
+#pragma unroll
+    for (int o = W / 2; o > 0; o >>= 1) s += __shfl_xor_sync(~0u, s, o);
+    return {m, s};
 }
 
 __device__ __forceinline__ const float *row_of(const nck_rows &q, int64_t r) {
@@ -359,13 +385,7 @@ __global__ void __launch_bounds__(256) k_rows_small(nck_rows q, nck_policy p, in
             }
 #pragma unroll
             for (int u = 0; u < P; u++) {
-                Stat st = {kNone, 0.0f};
-                take(st, v[u]);
-#pragma unroll
-                for (int o = G / 2; o > 0; o >>= 1) {
-                    const Stat b = {__shfl_xor_sync(~0u, st.m, o), __shfl_xor_sync(~0u, st.s, o)};
-                    st = join(st, b);
-                }
+                const Stat st = lanes_stat<G>(v[u]);
                 const int from = lane % R * G;
                 const Stat mine = {__shfl_sync(~0u, st.m, from), __shfl_sync(~0u, st.s, from)};
                 if (lane / R == it + u) own = mine;
@@ -686,8 +706,8 @@ void dispatch_small(nck_dev *d, const nck_rows *q, const nck_policy *p, const nc
     else if (q->V <= 32) launch_small<8, 4, 4>(d, q, p, g);
     else if (q->V <= 64) launch_small<16, 4, 4>(d, q, p, g);
     else if (q->V <= 128) launch_small<32, 4, 4>(d, q, p, g);
-    else if (q->V <= 256) launch_small<32, 8, 4>(d, q, p, g);
-    else launch_small<32, 16, 2>(d, q, p, g);
+    else if (q->V <= 256) launch_small<32, 8, 3>(d, q, p, g);
+    else launch_small<32, 16, 1>(d, q, p, g);
 }
 
 }  // namespace
