@@ -10,10 +10,11 @@
 // Many loads in flight are what both need. Rows of up to kSmallRow logits belong to 1 to 32 lanes with several
 // rows of a warp's run in flight (200000 rows of 61 logits, both passes: 51 us; a warp a row took 187); rows of some
 // thousand logits to a warp, the long ones to a block of 256 threads (8 vectors in flight a thread forward, 16
-// backward: 4 x 2048 rows of 50001 logits with half of the rows counted take 123 and 350 us, 0.82 and 2.46 GB at the
-// copy rate 125 and 375; with 4 vectors 128 and 376; 132 forward since its exponential is the exact one). A few very long rows are split among warps, and a second launch
-// joins the parts. Statistics of up to 32 rows wait in a warp's lanes, so that the double precision arithmetic of
-// the loss runs once for all of them and not once a row. Backward deals rows out as blocks end (uncounted rows cost
+// backward: 4 x 2048 rows of 50001 logits with half of the rows counted take 132 and 352 us, 0.82 and 2.46 GB at the
+// copy rate 125 and 375; with 4 vectors 138 and 376; 123 forward with the approximate exponential; a second set of
+// vectors fetched while the first is summed 140 to 196, as it costs blocks an SM). A few very long rows are split
+// among warps, and a second launch joins the parts. Statistics of up to 32 rows wait in a warp's lanes, so that the
+// double precision arithmetic of the loss runs once for all of them and not once a row. Backward deals rows out as blocks end (uncounted rows cost
 // a third, so dealing them out in advance leaves SMs idle: 418 us) and starts with the last long row, whose logits
 // the forward pass may have left in L2. Log probabilities and everything behind them that can cancel (log ratios,
 // sums over tokens and rows) are held in 64 bits; sums run in a fixed order.
@@ -93,7 +94,7 @@ struct Stat {
     float m, s; // running maximum, and the sum of exp(z - m)
 };
 
-// adds a maximum / sum pair to another; a side without finite values has s = 0
+// adds a maximum / sum pair to another; a side without finite values adds nothing
 __device__ __forceinline__ Stat join(Stat a, Stat b) {
     const float m = fmaxf(a.m, b.m), base = m == kNone ? 0.0f : m;
     float ea, eb;
@@ -262,8 +263,8 @@ __device__ __forceinline__ double policy_term(const nck_policy &p, const RowIn &
     const float lo = 1.0f - p.clip_low, hi = 1.0f + p.clip_high;
     const float held = fminf(fmaxf(ratio, lo), hi);
     const float gain = fminf(ratio * A, held * A);
-    const bool moves = A >= 0.0f ? ratio <= hi : ratio >= lo;
-    float term = isnan(ratio) ? ratio : -gain, f = moves ? -A * ratio : 0.0f;
+    const bool moves = A >= 0.0f ? ratio <= hi : ratio >= lo, lost = isnan(ratio) || isnan(A);
+    float term = lost ? ratio + A : -gain, f = lost ? ratio + A : moves ? -A * ratio : 0.0f;
     if (p.kl != 0.0f) {
         const float away = (float)((double)in.ref - lp), e = expm1f(away);
         term += p.kl * (e - away);

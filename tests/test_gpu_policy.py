@@ -147,6 +147,24 @@ def test_policy_rows_left_out_hold_anything(V):
             assert float(e.np(tl)) == 0.0 and not e.np(more).any() and not e.grad(tz).any()
 
 
+@pytest.mark.parametrize("V", [5, 40, 2000, 20000])
+@pytest.mark.parametrize("kl", [0.0, 0.1])
+def test_policy_nan_in_counted_rows_shows(V, kl):
+    """A counted row with a NaN (or +inf) logit, old log probability or advantage: the loss is NaN and so is the
+    row's whole gradient; the other rows have theirs."""
+    z, act, old, ref, adv = make(13, (6,), V)
+    _, _, dz, _, off, _ = policy(z, act, old, ref, adv, None, 0.2, 0.25, kl)
+    z[1, V // 2], z[2, V - 1], old[3], adv[4] = np.nan, np.inf, np.nan, np.nan
+    with Eng("b200") as e:
+        tz, tl, _ = run_policy(e, z, act, old, ref, adv, None, kl=kl)
+        assert e.L.nc_backward(tl) == 0
+        g = e.grad(tz)
+        assert np.isnan(float(e.np(tl))) and np.isnan(g[1:5]).all()
+        for i in (0, 5):
+            assert np.all(abs(g[i] - dz[i]) <= off[i])
+        assert e.ok(), e.err()
+
+
 @pytest.mark.parametrize("V", [33, 4000])
 @pytest.mark.parametrize("low", [-np.inf, np.finfo(np.float32).min])
 def test_policy_banned_and_extreme_logits(V, low):
