@@ -96,9 +96,9 @@ NC_API int nc_ext_cross_entropy_fwd_noalloc(const float *logits, const int32_t *
  * Address of t's element 0 in device memory (a view's own first element; strides as created), with host
  * writes pushed and pending values computed. The data is that of the context's stream: a reader or writer on
  * another stream orders itself after nc_ext_stream (an event, or nc_ext_synchronize) and before the next op.
- * write != 0 says that the caller will write through the address: host mirrors are dropped. The address
- * holds until t is released or, for a temporary, until nc_step_end. NULL when t is NULL or holds no data, or
- * the context has an error. */
+ * write != 0 says that the caller will write through the address: host mirrors are dropped and pending values
+ * that read t are computed first (ask again before each round of writes). The address holds until t is released
+ * or, for a temporary, until nc_step_end. NULL when t is NULL or holds no data, or the context has an error. */
 NC_API void *nc_ext_device_data(nc_tensor *t, int write);
 /* nc_backward from any f32 tensor y with dy as the gradient of it (same shape, any strides, same context)
  * instead of a scalar loss with gradient 1. dy is read, never written or kept. Returns the context status. */

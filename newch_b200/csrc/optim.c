@@ -512,7 +512,10 @@ static int move_state(nc_optim *o, nc_tensor *t, int put) {
     nc_ctx *ctx = o->ctx;
     if (ctx->status != NC_OK || !state_tensor_ok(o, t, put ? "optim_put_state" : "optim_get_state")) return ctx->status;
     state_upload_if_dirty(o);
-    if (!put) nc__dev_write(t);
+    if (!put) {
+        nc__deferred_flush(ctx); /* pending recipes may read the tensor */
+        nc__dev_write(t);
+    }
     float *val = (float *)nc__dev(t);
     if (ctx->status != NC_OK) return ctx->status;
     if (o->kind == OPT_ADAMW8) {

@@ -348,6 +348,20 @@ def test_state_copies_of_other_optimizers_and_refusals():
         assert e.L.nc_ext_optim_get_state(empty, e.t(np.zeros((2, 0), F))) == 0 and e.ok(), e.err()
 
 
+@pytest.mark.parametrize("eight", [True, False])
+def test_state_over_a_tensor_that_something_pending_reads(eight):
+    w = np.random.default_rng(9).standard_normal((3, 200)).astype(F)
+    vals = np.random.default_rng(10).standard_normal((2, 600)).astype(F)
+    with Eng("b200") as e:
+        t = e.param(w)
+        o = optimizer(e, [t], make="nc_ext_adamw8" if eight else "nc_adamw")
+        tv = e.t(vals)
+        want = e.np(e.check(e.L.nc_gelu(e.t(vals), 0)))
+        y = e.check(e.L.nc_gelu(tv, 0))
+        assert e.L.nc_ext_optim_get_state(o, tv) == 0, e.err()
+        assert np.array_equal(e.np(y), want) and not e.np(tv).any()
+
+
 def test_parameter_of_more_than_2_to_the_31_elements():
     """Offsets past 32 bits: the last elements of one parameter of 2^31 + 777."""
     import torch

@@ -368,6 +368,22 @@ def test_device_data_is_the_tensor():
         assert e.L.nc_ext_device_data(None, 0) is None
 
 
+def test_device_data_for_writing_computes_what_still_reads_the_tensor():
+    import torch
+
+    a = seeded(4, (300, 128))
+    with Eng("b200") as e:
+        t = e.t(a)
+        want = e.np(e.check(e.L.nc_gelu(e.t(a), 0)))
+        y = e.check(e.L.nc_gelu(t, 0))  # kept pending until something reads it
+        face = type("Face", (), {"__cuda_array_interface__": dict(shape=a.shape, typestr="<f4", data=(e.L.nc_ext_device_data(t, 1), False), version=2)})
+        e.L.nc_ext_synchronize(e.ctx)
+        torch.as_tensor(face(), device="cuda").zero_()
+        torch.cuda.synchronize()
+        assert np.array_equal(e.np(y), want)
+        assert not e.np(t).any()
+
+
 def test_inside_attention():
     """Fused projection -> norms and rotation -> the framework's attention, forward and backward, against torch in
     64 bits; the fused attention reads the rotated heads through slices and transposes."""
