@@ -273,12 +273,28 @@ static void plan_release_node(nc_ctx *ctx, nc_node *n, nc_tensor *loss, const bw
 
 nc_status nc_backward(nc_tensor *loss) { return nc_backward_ex(loss, 0, NULL, 0); }
 
+/* whether dy's memory is (part of) a gradient that the pass may write */
+static int plan_writes(const bw_plan *pl, const nc_tensor *dy) {
+    const nc_tensor *o = nc__owner((nc_tensor *)dy);
+    const char *a = (const char *)o->data, *b = a + o->bytes;
+    for (int k = 0; k < pl->order.n; k++) {
+        const nc_node *n = pl->order.v[k];
+        for (int i = 0; i < n->n_in; i++) {
+            const nc_tensor *g = n->in[i]->grad;
+            if (!g) continue;
+            const char *c = (const char *)g->data;
+            if (c < b && a < c + g->bytes) return 1;
+        }
+    }
+    return 0;
+}
+
 /* d loss / d loss at the start of a pass: 1, or dy (the gradient of y given by the caller). A y that some op
  * produced and that holds no gradient reads the context's constant 1, or the caller's buffer, in place (an alias
  * that owns nothing and is dropped when the pass ends: *lent = 1; a retained pass keeps the gradient 1, in a
- * buffer of its own). Otherwise 1 or dy is stored into a fresh buffer or added to what is there. Returns 0 on
+ * buffer of its own), unless the pass adds to that buffer. Otherwise 1 or dy is stored into a fresh buffer or added to what is there. Returns 0 on
  * failure. */
-static int seed_gradient(nc_ctx *ctx, nc_tensor *y, nc_tensor *dy, int retain, int *lent) {
+static int seed_gradient(nc_ctx *ctx, nc_tensor *y, nc_tensor *dy, const bw_plan *pl, int retain, int *lent) {
     *lent = 0;
     if (!dy && !retain && y->node && !y->grad) { /* the context's constant 1, the same for every pass */
         if (!ctx->one) {
@@ -292,7 +308,7 @@ static int seed_gradient(nc_ctx *ctx, nc_tensor *y, nc_tensor *dy, int retain, i
         *lent = 1;
         return 1;
     }
-    if (dy && y->node && !y->grad && nc_is_contiguous(dy)) {
+    if (dy && y->node && !y->grad && nc_is_contiguous(dy) && !plan_writes(pl, dy)) {
         nc__dev(dy);
         y->grad = nc__tensor_alias(dy, 0);
         *lent = y->grad != NULL;
@@ -380,7 +396,7 @@ static nc_status backward_pass(nc_tensor *loss, nc_tensor *dy, int flags, nc_ten
     }
 
     int lent;
-    if (!seed_gradient(ctx, loss, dy, retain, &lent)) {
+    if (!seed_gradient(ctx, loss, dy, &pl, retain, &lent)) {
         plan_free(&pl);
         return ctx->status;
     }

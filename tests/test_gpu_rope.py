@@ -279,6 +279,20 @@ def test_backward_from_is_backward_of_the_weighted_sum():
         assert np.array_equal(e.np(td), dy)
 
 
+def test_backward_from_the_gradient_of_a_leaf():
+    """dy is the gradient buffer of x, which the pass adds to: the pass reads dy as it was."""
+    x, w, first = seeded(1, (40, 24)), seeded(2, (24, 24)), seeded(3, (40, 24))
+    with Eng("b200") as e:
+        tx, tw = e.param(x), e.param(w)
+        assert e.L.nc_ext_backward_from(tx, e.t(first)) == 0  # x's gradient is `first`
+        y = e.check(e.L.nc_linear_fn(tx, tw, None))
+        assert e.L.nc_ext_backward_from(y, e.L.nc_grad(tx)) == 0, e.err()
+        x, w, first = (v.astype(np.float64) for v in (x, w, first))
+        # sums of 24 and 40 products: at most 40 roundings of the sum of absolute values (3xTF32 drops 2^-21 of each)
+        assert np.all(abs(e.grad(tw) - first.T @ x) <= (40 * E + 2.0 ** -20) * (abs(first).T @ abs(x)))
+        assert np.all(abs(e.grad(tx) - (first + first @ w)) <= (40 * E + 2.0 ** -20) * (abs(first) + abs(first) @ abs(w)))
+
+
 def test_backward_from_refuses():
     with Eng("b200") as e:
         p = e.param(seeded(1, (2, 3)))
