@@ -68,31 +68,42 @@ constexpr int kOwn = 4, kTwo = kOwn / 2; // pairs per lane, and their register p
 // 3 blocks of 1, 130 with 3 rows.
 constexpr int kRowsFwd = 4, kRowsBwd = 2;
 
-// The pairs of one row that a lane owns, kOwn / VEC vectors of VEC pairs: the first and the second elements of
-// each pair. Pairs behind the row's end read as zero.
+// Pairs in a lane's vector of VEC floats (two of them for split halves; with neighbours one vector holds both
+// elements of its pairs, and a float of its own is half a pair).
+template <int VEC, bool INTER>
+constexpr int kPairs = INTER ? (VEC > 1 ? VEC / 2 : 1) : VEC;
+
+// The pairs of one row that a lane owns, kOwn / kPairs vectors' worth: the first and the second elements of each pair.
+// Neighbouring lanes' vectors are neighbours, so that a load or store of a warp covers whole sectors. Neighbours as
+// pairs need sizes that are multiples of 4 only for float4 (two vectors a lane, 16 bytes apart, wrote each sector twice
+// and needed multiples of 8: forward 16 x 4000 x 16 heads of 20 57 us, now 40; both passes of 4 x 8000 x 8 heads of 100
+// 129 us, now 110; 24 x 1369 x 24 heads of 72 86 us, now 84.5).
+// Pairs behind the row's end read as zero.
 template <int VEC, int LPR, bool INTER>
 struct Own {
     float2 a[kTwo], b[kTwo];
-    static constexpr int NJ = kOwn / VEC;
+    static constexpr int P = kPairs<VEC, INTER>, NJ = kOwn / P;
     __device__ __forceinline__ void get(const float *row, int half, int l) {
         float x[kOwn], y[kOwn];
 #pragma unroll
         for (int j = 0; j < NJ; j++) {
-            const int p = (j * LPR + l) * VEC;
-            float u[VEC] = {}, v[VEC] = {};
-            if (p < half) {
-                load<VEC>(row + (INTER ? 2 * p : p), u);
-                load<VEC>(row + (INTER ? 2 * p + VEC : half + p), v);
-            }
-#pragma unroll
-            for (int i = 0; i < VEC; i++) {
-                if (INTER) { // u, v hold 2 VEC neighbours: pair i is elements 2i and 2i + 1
-                    x[j * VEC + i] = 2 * i < VEC ? u[(2 * i) % VEC] : v[(2 * i) % VEC];
-                    y[j * VEC + i] = 2 * i + 1 < VEC ? u[(2 * i + 1) % VEC] : v[(2 * i + 1) % VEC];
-                } else {
-                    x[j * VEC + i] = u[i];
-                    y[j * VEC + i] = v[i];
+            const int p = (j * LPR + l) * P;
+            if constexpr (INTER) {
+                float u[2 * P] = {};
+                if (p < half) {
+                    if constexpr (VEC == 1) u[0] = row[2 * p], u[1] = row[2 * p + 1];
+                    else load<2 * P>(row + 2 * p, u);
                 }
+#pragma unroll
+                for (int i = 0; i < P; i++) x[j * P + i] = u[2 * i], y[j * P + i] = u[2 * i + 1];
+            } else {
+                float u[P] = {}, v[P] = {};
+                if (p < half) {
+                    load<P>(row + p, u);
+                    load<P>(row + half + p, v);
+                }
+#pragma unroll
+                for (int i = 0; i < P; i++) x[j * P + i] = u[i], y[j * P + i] = v[i];
             }
         }
 #pragma unroll
@@ -102,17 +113,21 @@ struct Own {
         const float x[kOwn] = {a[0].x, a[0].y, a[1].x, a[1].y}, y[kOwn] = {b[0].x, b[0].y, b[1].x, b[1].y};
 #pragma unroll
         for (int j = 0; j < NJ; j++) {
-            const int p = (j * LPR + l) * VEC;
+            const int p = (j * LPR + l) * P;
             if (p >= half) continue;
-            float u[VEC], v[VEC];
+            if constexpr (INTER) {
+                float u[2 * P];
 #pragma unroll
-            for (int i = 0; i < VEC; i++) {
-                const int e = i, f = VEC + i; // INTER: elements e and f of the 2 VEC neighbours
-                u[i] = !INTER ? x[j * VEC + i] : e % 2 ? y[j * VEC + e / 2] : x[j * VEC + e / 2];
-                v[i] = !INTER ? y[j * VEC + i] : f % 2 ? y[j * VEC + f / 2] : x[j * VEC + f / 2];
+                for (int i = 0; i < P; i++) u[2 * i] = x[j * P + i], u[2 * i + 1] = y[j * P + i];
+                if constexpr (VEC == 1) row[2 * p] = u[0], row[2 * p + 1] = u[1];
+                else store<2 * P>(row + 2 * p, u);
+            } else {
+                float u[P], v[P];
+#pragma unroll
+                for (int i = 0; i < P; i++) u[i] = x[j * P + i], v[i] = y[j * P + i];
+                store<P>(row + p, u);
+                store<P>(row + half + p, v);
             }
-            store<VEC>(row + (INTER ? 2 * p : p), u);
-            store<VEC>(row + (INTER ? 2 * p + VEC : half + p), v);
         }
     }
     __device__ __forceinline__ void fill(float f) {
@@ -151,7 +166,7 @@ struct Turns {
         __syncthreads();
     }
     // cos and sin of the lane's pairs at token (b, t)
-    template <int VEC, int LPR>
+    template <int P, int LPR>
     __device__ __forceinline__ void at(const nck_rope &q, int64_t b, int64_t t, int l, float2 (&c)[kTwo], float2 (&s)[kTwo]) const {
         int pos[3] = {(int)t, 0, 0};
         if (q.pos) {
@@ -163,7 +178,7 @@ struct Turns {
         float cv[kOwn], sv[kOwn];
 #pragma unroll
         for (int i = 0; i < kOwn; i++) {
-            const int p = ((i / VEC * LPR + l) * VEC + i % VEC) & (NCK_ROPE_MAX_DIM / 2 - 1); // (behind the row: any)
+            const int p = ((i / P * LPR + l) * P + i % P) & (NCK_ROPE_MAX_DIM / 2 - 1); // (behind the row: any)
             const int a = axis[p];
             const int64_t at = a == 0 ? pos[0] : a == 1 ? pos[1] : pos[2];
             const int32_t turn = (int32_t)(((uint64_t)at * step[p]) >> 32);   // of 2^32
@@ -215,7 +230,7 @@ __global__ void __launch_bounds__(256, 2) k_rope_fwd(const __grid_constant__ nck
         for (int k = 0; k < U; k++)
             if (m.h0 + k < m.h1) row[k].get(x + k * q.sh, half, l);
         float2 c[kTwo], s[kTwo];
-        turns.template at<VEC, LPR>(q, m.b, m.t, l, c, s);
+        turns.template at<Row::P, LPR>(q, m.b, m.t, l, c, s);
         // y_a = r (x_a ac - x_b bs), y_b = r (x_b bc + x_a as), from the weight of the heads that follow
         float2 ac[kTwo], as[kTwo], bc[kTwo], bs[kTwo];
         const auto weigh = [&](const float *w) {
@@ -269,7 +284,7 @@ __global__ void __launch_bounds__(256, 2) k_rope_bwd(const __grid_constant__ nck
                                                   float *__restrict__ part) {
     constexpr int kPer = 32 / LPR, kGroups = 8 * kPer, U = VEC == 4 ? kRowsBwd : kRowsBwd - 1;
     typedef Own<VEC, LPR, INTER> Row;
-    __shared__ float red[kGroups * 2 * LPR * kOwn];
+    __shared__ __align__(16) float red[kGroups * 2 * LPR * kOwn]; // vectors are put there
     const int lane = threadIdx.x & 31, l = lane % LPR, half = q.D >> 1;
     const float inv_d = 1.0f / (float)q.D;
     __shared__ Turns turns;
@@ -290,7 +305,7 @@ __global__ void __launch_bounds__(256, 2) k_rope_bwd(const __grid_constant__ nck
         };
         fetch(m.h0);
         float2 c[kTwo], s[kTwo];
-        turns.template at<VEC, LPR>(q, m.b, m.t, l, c, s);
+        turns.template at<Row::P, LPR>(q, m.b, m.t, l, c, s);
         Row ws;
         const auto weigh = [&](const float *w) {
             if (w) ws.get(w, half, l);
@@ -392,10 +407,10 @@ __global__ void __launch_bounds__(1024) k_rope_dw(const float *__restrict__ part
 
 bool aligned(const void *p, int vec) { return ((uintptr_t)p & (size_t)(4 * vec - 1)) == 0; }
 
-// The widest vector that x's layout and every pointer of the pass allow: 4, 2 or 1 pairs.
+// The widest vector that x's layout and every pointer of the pass allow: 4, 2 or 1 floats.
 int vector_of(const nck_rope *q, const void *p1, const void *p2) {
     for (int vec = 4; vec > 1; vec >>= 1) {
-        bool ok = q->D % (2 * vec) == 0 && aligned(q->x, vec) && aligned(q->wq, vec) && aligned(q->wk, vec) &&
+        bool ok = q->D % (q->interleaved ? vec : 2 * vec) == 0 && aligned(q->x, vec) && aligned(q->wq, vec) && aligned(q->wk, vec) &&
                   aligned(p1, vec) && aligned(p2, vec);
         ok = ok && (q->B == 1 || q->sb % vec == 0) && (q->T == 1 || q->st % vec == 0) && (q->H == 1 || q->sh % vec == 0);
         if (ok) return vec;
