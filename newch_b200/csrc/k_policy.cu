@@ -445,7 +445,7 @@ __global__ void __launch_bounds__(256) k_rows_parts(nck_rows q, int parts, float
     for (int64_t it = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); it < q.N * parts; it += (int64_t)gridDim.x * 8) {
         const int64_t r = it / parts;
         if (!counted(q, r)) continue;
-        const Stat all = warp_join(read_row<32, 4>(row_of(q, r), q.V, lane, (int)(it - r * parts), parts));
+        const Stat all = warp_join(read_row<32, 8>(row_of(q, r), q.V, lane, (int)(it - r * parts), parts));
         if (lane == 0) part[it] = make_float2(all.m, all.s);
     }
 }
@@ -734,14 +734,16 @@ extern "C" void nck_rows_logp(nck_dev *d, const nck_rows *q, const nck_policy *p
         return;
     }
     wave_of(d, k_rows_block, &room_block);
-    // Parts of rows when the SMs would have less than two rows each and rows are long (of 128000 logits: 61 rows 15
-    // instead of 30 us, 122 23 for 31, 244 32 for 36, but 488 52 for 48; of 50001 61 rows 12.3 for 11.9).
-    if (q->N >= 2 * (int64_t)d->sm_count || q->V < 65536 || q->N == 0) {
+    // Parts of rows when an SM would have only a few rows and they are long, as the blocks that get one more row hold up
+    // the rest (parts and blocks, us: of 128000 logits 61 rows 15 and 30, 244 35 and 42, 488 52 and 59, 1464 125 and
+    // 130, 1952 169 and 166; of 256000 488 rows 89 and 108; of 65536 488 rows 35 and 35, 976 53 and 51; of 50001 61 rows
+    // 12.5 and 14).
+    if (q->V < 65536 || q->N >= d->sm_count * (q->V < 80000 ? (int64_t)2 : 10) || q->N == 0) {
         k_rows_block<<<at_most(q->N, room_block), 256, 0, NCK_STREAM(d)>>>(rows, pol, part, d->counters);
         return;
     }
     wave_of(d, k_rows_parts, &room_parts);
-    const int parts = parts_for(q->N, q->V, (int64_t)room_parts * 8 * 4, 2048);
+    const int parts = parts_for(q->N, q->V, (int64_t)room_parts * 8 * 2, 4096);
     float2 *stats = (float2 *)(part + 4096); // behind the finishing blocks' sums
     k_rows_parts<<<at_most((q->N * parts + 7) / 8, room_parts), 256, 0, NCK_STREAM(d)>>>(rows, parts, stats);
     cudaLaunchAttribute early;

@@ -15,7 +15,7 @@ pytestmark = pytest.mark.gpu
 
 SIZES = [(70, 4), (70, 5), (33, 8), (33, 9), (9, 16), (9, 17), (65, 32), (65, 33), (40, 64), (40, 65), (7, 128), (7, 129), (9, 255),
          (9, 256), (9, 257), (5, 512), (5, 513), (5, 900), (3, 2048), (3, 2049), (1100, 4099), (1023, 2051), (3, 12289),
-         (2, 65535), (7, 65537), (1, 200003), (297, 65536)]
+         (2, 65535), (7, 65537), (1, 200003), (297, 65536), (400, 80003)]
 
 
 @pytest.mark.parametrize("N,V", SIZES)
