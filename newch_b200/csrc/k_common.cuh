@@ -55,6 +55,21 @@ inline int resident_blocks(const nck_dev *d, K kernel, int threads, size_t smem 
     return per_sm * (d->sm_count > 0 ? d->sm_count : 148);
 }
 
+// A launch whose blocks may take their places while the kernel before it in the stream ends (2 to 3 us of a step of
+// two kernels). The kernel calls cudaGridDependencySynchronize before it reads or writes device memory: it returns
+// when everything before the kernel in the stream is done. Its loads are plain ones, never __ldg or by const
+// __restrict__ pointers: those promise memory that nothing writes from the kernel's start on, which is earlier.
+template <typename... P, typename... A>
+inline void launch_early(nck_dev *d, void (*kernel)(P...), int64_t grid, int threads, A... args) {
+    cudaLaunchAttribute early;
+    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    early.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = (unsigned)grid, cfg.blockDim = (unsigned)threads, cfg.stream = (cudaStream_t)d->stream;
+    cfg.attrs = &early, cfg.numAttrs = 1;
+    cudaLaunchKernelEx(&cfg, kernel, P(args)...);
+}
+
 // A block's walk over the items of one channel in an [N][C][S] tensor: planes [n0, n1) of channel c,
 // SV vector items per plane. Thread t takes items t, t + B, t + 2B, ... (B = blockDim.x) and advances
 // its (plane, item) pair by a carry instead of a division per item.

@@ -17,9 +17,10 @@
 // elements. A warp owns a block: a lane holds eight elements as two float4 of w and of g and the sixteen codes
 // of them as one 16-byte word (the codes are stored in that order), the largest values are a warp's maximum, and
 // nothing is read or written twice. A code's proposal is biased upward by 2^-20 of the root (the approximate
-// root is off by 2^-22 at most), so one border settles it. Measured on 135M weights (2.16 GB a step): 363 us, 91% of the measured copy rate; with two-sided
-// borders, denormal-safe roots and separate code arrays (116 issue slots an element) it was 560 us. The step itself is formed with the approximate division and root (each within 2 steps of fp32 of a term
-// that is lr times w's size or less).
+// root is off by 2^-22 at most), so one border settles it. Measured on 135M weights (2.16 GB a step): 360 us, 92% of
+// the measured copy rate; with two-sided borders, denormal-safe roots and separate code arrays (116 issue slots an
+// element) it was 560 us. The step itself is formed with the approximate division and root (each within 2 steps of
+// fp32 of a term that is lr times w's size or less).
 #include "k_common.cuh"
 
 using namespace nck;
@@ -143,8 +144,9 @@ struct Step8 {
     float gs, keep, beta1, up1, beta2, up2, rate, unbias2, eps;
 };
 
-__global__ void __launch_bounds__(256) k_adamw8(Step8 h, nck_opt8 q, const nck_opt8_chunk *__restrict__ chunks,
-                                                const unsigned char *__restrict__ present) {
+__global__ void __launch_bounds__(256) k_adamw8(Step8 h, nck_opt8 q, const nck_opt8_chunk *chunks,
+                                                const unsigned char *present) {
+    cudaGridDependencySynchronize();
     const nck_opt8_chunk c = chunks[blockIdx.x];
     if (present && !present[c.param]) return;
     const int lane = threadIdx.x & 31, off = (int)(threadIdx.x >> 5) * kBlock, n = c.len - off;
@@ -177,13 +179,13 @@ __global__ void __launch_bounds__(256) k_adamw8(Step8 h, nck_opt8 q, const nck_o
     if (lane == 0) *tops = top;
 }
 
-// The values of one moment of a block (its 4-byte groups of codes `step` 16-byte words apart): float4 stores at
-// 16-byte boundaries wherever `to` starts, so that a row of moments may begin at any element.
+// The values of one moment of a block: float4 stores at 16-byte boundaries wherever `to` starts, so that a row of
+// moments may begin at any element (135M weights' two moments 226 us, 1.35 GB; 240 with loads and stores in turn).
 template <bool M>
 __device__ __forceinline__ void emit(const uint32_t *codes, float *to, int n, float s, int lane) {
     const float unit = s * (M ? kUnitM : kUnitV);
     const uint32_t *mine = codes + (M ? 0 : 2);
-    const auto group = [&](int g) { return __ldg(mine + (g & 31) * 4 + (g >> 5)); }; // codes of elements 4g .. 4g + 3
+    const auto group = [&](int g) { return mine[(g & 31) * 4 + (g >> 5)]; }; // codes of elements 4g .. 4g + 3
     const auto value = [&](uint32_t w, int k) { return M ? decode_m(w, k, s, unit) : decode_v(w, k, s, unit); };
     if (n < kBlock) {
         for (int e = lane; e < n; e += 32) {
@@ -193,25 +195,30 @@ __device__ __forceinline__ void emit(const uint32_t *codes, float *to, int n, fl
         return;
     }
     const int lead = (int)((16 - ((uintptr_t)to & 15)) & 15) >> 2; // elements before the first boundary
+    uint32_t words[2]; // both on their way before anything is stored
+#pragma unroll
+    for (int k = 0; k < 2; k++) {
+        const int g = lane + 32 * k;
+        words[k] = !lead ? group(g) : g < 63 ? __funnelshift_r(group(g), group(g + 1), 8 * lead) : 0;
+    }
+    const int e = lane < lead ? lane : kBlock - 4 + lane; // elements before the first and behind the last boundary
+    const uint32_t end = lead && lane < 4 ? group(e >> 2) >> (8 * (e & 3)) : 0;
 #pragma unroll
     for (int k = 0; k < 2; k++) {
         const int g = lane + 32 * k;
         if (lead && g == 63) break;
-        const uint32_t w = lead ? __funnelshift_r(group(g), group(g + 1), 8 * lead) : group(g);
+        const uint32_t w = words[k];
         *reinterpret_cast<float4 *>(to + lead + 4 * g) = make_float4(value(w, 0), value(w, 1), value(w, 2), value(w, 3));
     }
-    if (lead && lane < 4) { // the elements before the first and behind the last boundary
-        const int e = lane < lead ? lane : kBlock - 4 + lane;
-        const uint32_t w = group(e >> 2) >> (8 * (e & 3));
-        to[e] = value(w, 0);
-    }
+    if (lead && lane < 4) to[e] = value(end, 0);
 }
 
 // Codes to values (PUT false) or values to codes: m's at val[0], v's at val[second], a span's at its offset.
 template <bool PUT>
-__global__ void __launch_bounds__(256) k_opt8_values(nck_opt8 q, const nck_opt8_span *__restrict__ spans,
-                                                     const nck_opt_chunk *__restrict__ chunks, float *val, int64_t second,
+__global__ void __launch_bounds__(256) k_opt8_values(nck_opt8 q, const nck_opt8_span *spans,
+                                                     const nck_opt_chunk *chunks, float *val, int64_t second,
                                                      int dense) {
+    cudaGridDependencySynchronize();
     const nck_opt_chunk c = chunks[blockIdx.x];
     const nck_opt8_span s = spans[c.seg];
     const int lane = threadIdx.x & 31, off = (int)(threadIdx.x >> 5) * kBlock;
@@ -265,7 +272,7 @@ extern "C" void nck_adamw8_step(nck_dev *d, const nck_opt_hyper *h, const nck_op
     s.rate = h->lr / h->bc1;
     s.unbias2 = 1.0f / sqrtf(h->bc2);
     s.eps = h->eps;
-    k_adamw8<<<nchunk, 256, 0, NCK_STREAM(d)>>>(s, *q, dchunks, present);
+    launch_early(d, k_adamw8, nchunk, 256, s, *q, dchunks, present);
     NCK_LAUNCHED(d, 1);
 }
 
@@ -273,7 +280,7 @@ extern "C" void nck_opt8_values(nck_dev *d, const nck_opt8 *q, const nck_opt8_sp
                                 int nchunk, int64_t total, float *val, int64_t second, int dense, int put) {
     if (nchunk <= 0) return;
     Scope sc(d, put ? "opt8_put" : "opt8_get", 0.0, 10.0 * total);
-    if (put) k_opt8_values<true><<<nchunk, 256, 0, NCK_STREAM(d)>>>(*q, dspans, dchunks, val, second, dense);
-    else k_opt8_values<false><<<nchunk, 256, 0, NCK_STREAM(d)>>>(*q, dspans, dchunks, val, second, dense);
+    if (put) launch_early(d, k_opt8_values<true>, nchunk, 256, *q, dspans, dchunks, val, second, dense);
+    else launch_early(d, k_opt8_values<false>, nchunk, 256, *q, dspans, dchunks, val, second, dense);
     NCK_LAUNCHED(d, 1);
 }

@@ -145,7 +145,7 @@ __device__ __forceinline__ Stat read_row(const float *z, int64_t V, int t, int k
         float4 f[U];
         float v[4 * U];
 #pragma unroll
-        for (int u = 0; u < U; u++) f[u] = __ldg(z4 + i + u * W);
+        for (int u = 0; u < U; u++) f[u] = z4[i + u * W];
 #pragma unroll
         for (int u = 0; u < U; u++) v[4 * u] = f[u].x, v[4 * u + 1] = f[u].y, v[4 * u + 2] = f[u].z, v[4 * u + 3] = f[u].w;
         take(st, v);
@@ -153,7 +153,7 @@ __device__ __forceinline__ Stat read_row(const float *z, int64_t V, int t, int k
     if (i < end) { // the rest, at most U - 1 vectors a thread
         float4 f[U - 1 > 0 ? U - 1 : 1];
 #pragma unroll
-        for (int u = 0; u < U - 1; u++) f[u] = i + u * W < end ? __ldg(z4 + i + u * W) : make_float4(kNone, kNone, kNone, kNone);
+        for (int u = 0; u < U - 1; u++) f[u] = i + u * W < end ? z4[i + u * W] : make_float4(kNone, kNone, kNone, kNone);
 #pragma unroll
         for (int u = 0; u < U - 1; u++) {
             const float v[4] = {f[u].x, f[u].y, f[u].z, f[u].w};
@@ -178,7 +178,7 @@ __device__ __forceinline__ Stat read_short_row(const float *z, int V, int lane) 
     const float v0[2] = {lane < lead ? z[lane] : kNone, lane < V - tail ? z[tail + lane] : kNone};
 #pragma unroll
     for (int u = 0; u < U; u++)
-        f[u] = lane + 32 * u < nv ? __ldg(z4 + lane + 32 * u) : make_float4(kNone, kNone, kNone, kNone);
+        f[u] = lane + 32 * u < nv ? z4[lane + 32 * u] : make_float4(kNone, kNone, kNone, kNone);
     Stat st = {kNone, 0.0f};
     take(st, v0);
 #pragma unroll
@@ -333,6 +333,7 @@ __device__ void finish_loss(const nck_policy &p, Sums mine, double2 *part, unsig
 
 // One warp a run of `run` rows, row i's statistics in lane i.
 __global__ void __launch_bounds__(256) k_rows_warp(nck_rows q, nck_policy p, int run, double2 *part, unsigned *counter) {
+    cudaGridDependencySynchronize();
     const int lane = threadIdx.x & 31;
     const int64_t warps = (int64_t)gridDim.x * 8;
     Sums sums = {0.0, 0.0};
@@ -363,6 +364,7 @@ __global__ void __launch_bounds__(256) k_rows_warp(nck_rows q, nck_policy p, int
 // statistics go to lane i.
 template <int G, int E, int P>
 __global__ void __launch_bounds__(256) k_rows_small(nck_rows q, nck_policy p, int run, double2 *part, unsigned *counter) {
+    cudaGridDependencySynchronize();
     constexpr int R = 32 / G;
     const int lane = threadIdx.x & 31, l = lane % G, V = (int)q.V;
     const int64_t warps = (int64_t)gridDim.x * 8;
@@ -382,7 +384,7 @@ __global__ void __launch_bounds__(256) k_rows_small(nck_rows q, nck_policy p, in
                 const bool ok = row < n && (any >> row & 1);
                 const float *z = row_of(q, r0 + (ok ? row : 0));
 #pragma unroll
-                for (int e = 0; e < E; e++) v[u][e] = ok && e * G + l < V ? __ldg(z + e * G + l) : kNone;
+                for (int e = 0; e < E; e++) v[u][e] = ok && e * G + l < V ? z[e * G + l] : kNone;
             }
 #pragma unroll
             for (int u = 0; u < P; u++) {
@@ -404,6 +406,7 @@ __global__ void __launch_bounds__(256) k_rows_small(nck_rows q, nck_policy p, in
 
 // A block a row. Statistics of counted rows wait in the lanes of the first warp, which finishes 32 at a time.
 __global__ void __launch_bounds__(256) k_rows_block(nck_rows q, nck_policy p, double2 *part, unsigned *counter) {
+    cudaGridDependencySynchronize();
     __shared__ Stat red[2][8];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     Sums sums = {0.0, 0.0};
@@ -441,6 +444,7 @@ __global__ void __launch_bounds__(256) k_rows_block(nck_rows q, nck_policy p, do
 
 // Few rows: a warp takes parts of rows, with no barrier between warps; k_rows_finish joins them.
 __global__ void __launch_bounds__(256) k_rows_parts(nck_rows q, int parts, float2 *part) {
+    cudaGridDependencySynchronize();
     const int lane = threadIdx.x & 31;
     for (int64_t it = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); it < q.N * parts; it += (int64_t)gridDim.x * 8) {
         const int64_t r = it / parts;
@@ -453,7 +457,7 @@ __global__ void __launch_bounds__(256) k_rows_parts(nck_rows q, int parts, float
 // A warp a run of rows: their parts joined, row i's in lane i, and the rows finished.
 __global__ void __launch_bounds__(256) k_rows_finish(nck_rows q, nck_policy p, int parts, int run, const float2 *part,
                                                      double2 *sums_of, unsigned *counter) {
-    cudaGridDependencySynchronize(); // launched early: the parts are there when the kernel before has ended
+    cudaGridDependencySynchronize();
     const int lane = threadIdx.x & 31;
     Sums sums = {0.0, 0.0};
     const int64_t r0 = ((int64_t)blockIdx.x * 8 + (threadIdx.x >> 5)) * run;
@@ -483,7 +487,8 @@ __global__ void __launch_bounds__(256) k_rows_finish(nck_rows q, nck_policy p, i
 }
 
 // Sums of a pair's two sequences, the pair's loss term and its sequences' factors; the last block sums the terms.
-__global__ void __launch_bounds__(256) k_pairs(nck_pairs p, const double *__restrict__ lp, double *term, unsigned *counter) {
+__global__ void __launch_bounds__(256) k_pairs(nck_pairs p, const double *lp, double *term, unsigned *counter) {
+    cudaGridDependencySynchronize();
     __shared__ double red[2][8];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int64_t i = blockIdx.x;
@@ -556,7 +561,7 @@ __device__ __forceinline__ void grad_row(const float *z, float *dst, int64_t V, 
     const int64_t hot = a - lead; // the label's place among the vectors' floats
     const auto fetch = [&](int j) {
         const float *at = from + 4 * (int64_t)j;
-        return even ? __ldg(reinterpret_cast<const float4 *>(at)) : make_float4(__ldg(at), __ldg(at + 1), __ldg(at + 2), __ldg(at + 3));
+        return even ? *reinterpret_cast<const float4 *>(at) : make_float4(at[0], at[1], at[2], at[3]);
     };
     const auto give = [&](int j, float4 v, float4 old) {
         float4 g = make_float4(f * exp_of(v.x - m), f * exp_of(v.y - m), f * exp_of(v.z - m), f * exp_of(v.w - m));
@@ -581,6 +586,7 @@ __device__ __forceinline__ void grad_row(const float *z, float *dst, int64_t V, 
 
 template <int W, bool ACC>
 __global__ void __launch_bounds__(256) k_rows_grad(nck_rows q, nck_rows_grad g, int parts) {
+    cudaGridDependencySynchronize();
     const int t = threadIdx.x % W;
     const float up = g.up[0] * (g.scale ? g.scale[0] : 1.0f);
     const int64_t teams = (int64_t)gridDim.x * (256 / W);
@@ -599,6 +605,7 @@ __global__ void __launch_bounds__(256) k_rows_grad(nck_rows q, nck_rows_grad g, 
 template <int G, int E, int P, bool ACC>
 __global__ void __launch_bounds__(256) k_rows_grad_small(nck_rows q, nck_rows_grad g, int run) {
     constexpr int R = 32 / G;
+    cudaGridDependencySynchronize();
     const int lane = threadIdx.x & 31, l = lane % G, V = (int)q.V;
     const float up = g.up[0] * (g.scale ? g.scale[0] : 1.0f);
     const int64_t r0 = ((int64_t)blockIdx.x * 8 + (threadIdx.x >> 5)) * run;
@@ -627,7 +634,7 @@ __global__ void __launch_bounds__(256) k_rows_grad_small(nck_rows q, nck_rows_gr
             const float *dz = g.dz + (r0 + (ok ? row : 0)) * V;
 #pragma unroll
             for (int e = 0; e < E; e++) {
-                v[u][e] = read && e * G + l < V ? __ldg(z + e * G + l) : kNone;
+                v[u][e] = read && e * G + l < V ? z[e * G + l] : kNone;
                 if (ACC) old[ACC ? u : 0][ACC ? e : 0] = read && e * G + l < V ? dz[e * G + l] : 0.0f;
             }
         }
@@ -671,7 +678,7 @@ void launch_grad(nck_dev *d, const nck_rows *q, const nck_rows_grad *g) {
     static int room = 0;
     wave_of(d, k_rows_grad<W, ACC>, &room);
     const int parts = W == 32 ? 1 : parts_for(q->N, q->V, room, 4096);
-    k_rows_grad<W, ACC><<<at_most((q->N * parts + 256 / W - 1) / (256 / W), 1 << 30), 256, 0, NCK_STREAM(d)>>>(*q, *g, parts);
+    launch_early(d, k_rows_grad<W, ACC>, at_most((q->N * parts + 256 / W - 1) / (256 / W), 1 << 30), 256, *q, *g, parts);
     NCK_LAUNCHED(d, 1);
 }
 
@@ -693,9 +700,9 @@ void launch_small(nck_dev *d, const nck_rows *q, const nck_policy *p, const nck_
     constexpr int R = 32 / G;
     const int run = (run_for(d, q->N, room) + R - 1) / R * R; // whole passes
     const int64_t blocks = (q->N + run * 8 - 1) / (run * 8);
-    if (p) k_rows_small<G, E, P><<<at_most(blocks, room), 256, 0, NCK_STREAM(d)>>>(*q, *p, run, (double2 *)d->scratch, d->counters);
-    else if (g->acc) k_rows_grad_small<G, E, P, true><<<(unsigned)blocks, 256, 0, NCK_STREAM(d)>>>(*q, *g, run);
-    else k_rows_grad_small<G, E, P, false><<<(unsigned)blocks, 256, 0, NCK_STREAM(d)>>>(*q, *g, run);
+    if (p) launch_early(d, k_rows_small<G, E, P>, at_most(blocks, room), 256, *q, *p, run, (double2 *)d->scratch, d->counters);
+    else if (g->acc) launch_early(d, k_rows_grad_small<G, E, P, true>, blocks, 256, *q, *g, run);
+    else launch_early(d, k_rows_grad_small<G, E, P, false>, blocks, 256, *q, *g, run);
     NCK_LAUNCHED(d, 1);
 }
 
@@ -729,8 +736,7 @@ extern "C" void nck_rows_logp(nck_dev *d, const nck_rows *q, const nck_policy *p
     NCK_LAUNCHED(d, 1);
     if (warp_rows(q)) {
         const int64_t run = run_for(d, q->N, wave_of(d, k_rows_warp, &room_warp));
-        k_rows_warp<<<at_most((q->N + run * 8 - 1) / (run * 8), room_warp), 256, 0, NCK_STREAM(d)>>>(rows, pol, (int)run, part,
-                                                                                                 d->counters);
+        launch_early(d, k_rows_warp, at_most((q->N + run * 8 - 1) / (run * 8), room_warp), 256, rows, pol, (int)run, part, d->counters);
         return;
     }
     wave_of(d, k_rows_block, &room_block);
@@ -739,27 +745,22 @@ extern "C" void nck_rows_logp(nck_dev *d, const nck_rows *q, const nck_policy *p
     // 130, 1952 169 and 166; of 256000 488 rows 89 and 108; of 65536 488 rows 35 and 35, 976 53 and 51; of 50001 61 rows
     // 12.5 and 14).
     if (q->V < 65536 || q->N >= d->sm_count * (q->V < 80000 ? (int64_t)2 : 10) || q->N == 0) {
-        k_rows_block<<<at_most(q->N, room_block), 256, 0, NCK_STREAM(d)>>>(rows, pol, part, d->counters);
+        launch_early(d, k_rows_block, at_most(q->N, room_block), 256, rows, pol, part, d->counters);
         return;
     }
     wave_of(d, k_rows_parts, &room_parts);
     const int parts = parts_for(q->N, q->V, (int64_t)room_parts * 8 * 2, 4096);
     float2 *stats = (float2 *)(part + 4096); // behind the finishing blocks' sums
-    k_rows_parts<<<at_most((q->N * parts + 7) / 8, room_parts), 256, 0, NCK_STREAM(d)>>>(rows, parts, stats);
-    cudaLaunchAttribute early;
-    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    early.val.programmaticStreamSerializationAllowed = 1;
-    cudaLaunchConfig_t cfg = {};
+    launch_early(d, k_rows_parts, at_most((q->N * parts + 7) / 8, room_parts), 256, rows, parts, stats);
     const int64_t run = (q->N + 4096 * 8 - 1) / (4096 * 8); // (few rows: one)
-    cfg.gridDim = (unsigned)((q->N + run * 8 - 1) / (run * 8)), cfg.blockDim = 256, cfg.stream = NCK_STREAM(d);
-    cfg.attrs = &early, cfg.numAttrs = 1;
-    cudaLaunchKernelEx(&cfg, k_rows_finish, rows, pol, parts, (int)run, (const float2 *)stats, part, d->counters);
+    launch_early(d, k_rows_finish, (q->N + run * 8 - 1) / (run * 8), 256, rows, pol, parts, (int)run, (const float2 *)stats, part,
+                 d->counters);
     NCK_LAUNCHED(d, 1);
 }
 
 extern "C" void nck_pref_pairs(nck_dev *d, const nck_pairs *p, const double *lp) {
     Scope sc(d, "preference_pairs", 0.0, 16.0 * p->P * p->T);
-    k_pairs<<<(unsigned)p->P, 256, 0, NCK_STREAM(d)>>>(*p, lp, p->term, d->counters);
+    launch_early(d, k_pairs, p->P, 256, *p, lp, p->term, d->counters);
     NCK_LAUNCHED(d, 1);
 }
 

@@ -221,6 +221,7 @@ __global__ void __launch_bounds__(256, 2) k_rope_fwd(const __grid_constant__ nck
     const float inv_d = 1.0f / (float)q.D;
     __shared__ Turns turns;
     turns.fill(q);
+    cudaGridDependencySynchronize();
     for (int64_t it = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); it < g.items; it += (int64_t)gridDim.x * 8) {
         const Item<LPR> m(q, g, it, lane / LPR);
         const float *x = q.x + m.b * q.sb + m.t * q.st + m.h0 * q.sh;
@@ -280,7 +281,7 @@ __global__ void __launch_bounds__(256, 2) k_rope_fwd(const __grid_constant__ nck
 // part (may be NULL): the block's sums of g n over its query rows and over its key rows, [block][2][D]
 template <int VEC, int LPR, bool INTER>
 __global__ void __launch_bounds__(256, 2) k_rope_bwd(const __grid_constant__ nck_rope q, const RopeGrid g,
-                                                  const float *__restrict__ dy, float *dx, int acc,
+                                                  const float *dy, float *dx, int acc,
                                                   float *__restrict__ part) {
     constexpr int kPer = 32 / LPR, kGroups = 8 * kPer, U = VEC == 4 ? kRowsBwd : kRowsBwd - 1;
     typedef Own<VEC, LPR, INTER> Row;
@@ -289,6 +290,7 @@ __global__ void __launch_bounds__(256, 2) k_rope_bwd(const __grid_constant__ nck
     const float inv_d = 1.0f / (float)q.D;
     __shared__ Turns turns;
     turns.fill(q);
+    cudaGridDependencySynchronize();
     Row sum[2]; // of query heads, of key heads
     sum[0].fill(0.0f), sum[1].fill(0.0f);
     for (int64_t it = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); it < g.items; it += (int64_t)gridDim.x * 8) {
@@ -375,10 +377,10 @@ __global__ void __launch_bounds__(256, 2) k_rope_bwd(const __grid_constant__ nck
 }
 
 // dw (+)= the blocks' partial sums in a fixed order; 32 columns a block, 32 slices of the blocks each
-__global__ void __launch_bounds__(1024) k_rope_dw(const float *__restrict__ part, int blocks, int D, float *dwq, int acc_q,
+__global__ void __launch_bounds__(1024) k_rope_dw(const float *part, int blocks, int D, float *dwq, int acc_q,
                                                   float *dwk, int acc_k) {
     __shared__ double red[32][33];
-    cudaGridDependencySynchronize(); // launched early: the sums are written when the kernel before has ended
+    cudaGridDependencySynchronize();
     const int lane = threadIdx.x & 31, sl = threadIdx.x >> 5, col = blockIdx.x * 32 + lane;
     double t = 0.0;
     if (col < 2 * D) {
@@ -443,8 +445,8 @@ int launch(nck_dev *d, const nck_rope *q, float *y, const float *dy, float *dx, 
     const RopeGrid g = split_of(d, q, LPR);
     const int64_t blocks = (g.items + 7) / 8;
     const int room = y ? room_fwd : room_bwd, grid = (int)(blocks < room ? blocks : room);
-    if (y) k_rope_fwd<VEC, LPR, INTER><<<grid, 256, 0, NCK_STREAM(d)>>>(*q, g, y);
-    else k_rope_bwd<VEC, LPR, INTER><<<grid, 256, 0, NCK_STREAM(d)>>>(*q, g, dy, dx, acc, part);
+    if (y) launch_early(d, k_rope_fwd<VEC, LPR, INTER>, grid, 256, *q, g, y);
+    else launch_early(d, k_rope_bwd<VEC, LPR, INTER>, grid, 256, *q, g, dy, dx, acc, part);
     NCK_LAUNCHED(d, 1);
     return grid;
 }
@@ -494,12 +496,6 @@ extern "C" void nck_rope_bwd(nck_dev *d, const nck_rope *q, const float *dy, flo
         grid = q->interleaved ? dispatch<true>(d, q, nullptr, dy, dx, acc_x, part)
                               : dispatch<false>(d, q, nullptr, dy, dx, acc_x, part);
     if (!part) return;
-    cudaLaunchAttribute early;
-    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    early.val.programmaticStreamSerializationAllowed = 1;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = (2 * q->D + 31) / 32, cfg.blockDim = 1024, cfg.stream = NCK_STREAM(d);
-    cfg.attrs = &early, cfg.numAttrs = grid > 0;
-    cudaLaunchKernelEx(&cfg, k_rope_dw, (const float *)part, grid, q->D, dwq, acc_q, dwk, acc_k);
+    launch_early(d, k_rope_dw, (2 * q->D + 31) / 32, 1024, (const float *)part, grid, q->D, dwq, acc_q, dwk, acc_k);
     NCK_LAUNCHED(d, 1);
 }
