@@ -158,3 +158,46 @@ def test_two_contexts_at_once():
         for e, s in ((a, sa), (b, sb)):
             for u, v in zip(end(e, *s), alone):
                 assert np.array_equal(u, v)
+
+
+@pytest.mark.parametrize("rows", [8, 100, 400, 1600, 8 * 200 * 6])
+def test_steps_back_to_back_are_steps_one_by_one(rows):
+    """Kernels take their places while the one before ends, and each reads what that one wrote (rows of 76800 to 64
+    logits: every way the losses run): 25 steps without a pause give the weights and moments of 25 steps with the host
+    waiting after every call, bit for bit."""
+    x, wt = seeded(1, (8, 200, 6, 64)), seeded(2, (64,)) + 1
+    V = x.size // rows
+    rng = np.random.default_rng(3)
+    act, adv = rng.integers(0, V, rows).astype(np.int32), seeded(4, (rows,))
+    old, mask = np.full(rows, -np.log(V), np.float32), (rng.random(rows) < 0.8).astype(np.int32)
+    ro, po = capi.RopeOpts(4, 1, (ctypes.c_int * 3)(32), 10000.0, 1e-6, 0), capi.PolicyOpts(0.2, 0.2, 0.0)
+
+    def run(pause):
+        with Eng("b200") as e:
+            wait = (lambda: e.L.nc_ext_synchronize(e.ctx)) if pause else (lambda: None)
+            e.L.nc_persistent_begin(e.ctx)
+            fixed = [e.t(v) for v in (act, old, adv, mask)]
+            state = e.t(np.zeros((2, x.size + 64), np.float32))
+            e.L.nc_persistent_end(e.ctx)
+            tx, tw = e.param(x), e.param(wt)
+            o = e.check(e.L.nc_ext_adamw8(e.ctx, capi.ptr_array([tx, tw]), 2, capi.OptimOpts(1e-2, 0.0, 0.01, 0.9, 0.999, 1e-8)))
+            for _ in range(25):
+                y = e.check(e.L.nc_ext_qk_norm_rope(tx, tw, tw, None, ctypes.byref(ro)))
+                wait()
+                z = e.check(e.L.nc_reshape(y, *capi.shape_arg((rows, V))))
+                loss = e.check(e.L.nc_ext_policy_loss(z, fixed[0], fixed[1], None, fixed[2], fixed[3], ctypes.byref(po), None))
+                wait()
+                e.L.nc_optim_clear_grad(o)
+                assert e.L.nc_backward_ex(loss, 1, None, 0) == 0, e.err()
+                wait()
+                e.L.nc_optim_step(o)
+                wait()
+                assert e.L.nc_ext_optim_get_state(o, state) == 0, e.err()
+                wait()
+                e.step_end()
+            out = [e.np(t) for t in (tx, tw, state)]
+            e.L.nc_optim_free(o)
+            return out
+
+    for a, b in zip(run(True), run(False)):
+        assert np.isfinite(a).all() and np.array_equal(a, b)
