@@ -10,14 +10,15 @@
 // Many loads in flight are what both need. Rows of up to kSmallRow logits belong to 1 to 32 lanes with several
 // rows of a warp's run in flight (200000 rows of 61 logits, both passes: 51 us; a warp a row took 187); rows of some
 // thousand logits to a warp, the long ones to a block of 256 threads (8 vectors in flight a thread forward, 16
-// backward: 4 x 2048 rows of 50001 logits with half of the rows counted take 132 and 352 us, 0.82 and 2.46 GB at the
-// copy rate 125 and 375; with 4 vectors 138 and 376; 123 forward with the approximate exponential; a second set of
-// vectors fetched while the first is summed 140 to 196, as it costs blocks an SM). A few very long rows are split
-// among warps, and a second launch joins the parts. Statistics of up to 32 rows wait in a warp's lanes, so that the
-// double precision arithmetic of the loss runs once for all of them and not once a row. Backward deals rows out as blocks end (uncounted rows cost
-// a third, so dealing them out in advance leaves SMs idle: 418 us) and starts with the last long row, whose logits
-// the forward pass may have left in L2. Log probabilities and everything behind them that can cancel (log ratios,
-// sums over tokens and rows) are held in 64 bits; sums run in a fixed order.
+// backward: 4096 rows of 50001 logits 151 and 252 us, 0.82 and 1.64 GB at the copy rate 125 and 250; forward 5 to 30%
+// longer with 4 vectors, with a second set of vectors fetched while the first is summed, or with the logits brought to
+// shared memory by bulk copies, as each leaves fewer warps to the arithmetic; 139 with the approximate exponential).
+// A few very long rows are split among warps, and a second launch joins the parts. Statistics of up to 32 rows wait in
+// a warp's lanes, so that the double precision arithmetic of the loss runs once for all of them and not once a row.
+// Backward deals rows out as blocks end (uncounted rows cost a third, so dealing them out in advance leaves SMs idle:
+// with a mask 418 instead of 352 us) and starts with the last long row, whose logits the forward pass may have left in
+// L2. Log probabilities and everything behind them that can cancel (log ratios, sums over tokens and rows) are held in
+// 64 bits; sums run in a fixed order.
 #include <math.h>
 
 #include "k_common.cuh"
