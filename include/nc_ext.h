@@ -101,7 +101,9 @@ NC_API int nc_ext_cross_entropy_fwd_noalloc(const float *logits, const int32_t *
  * or, for a temporary, until nc_step_end. NULL when t is NULL or holds no data, or the context has an error. */
 NC_API void *nc_ext_device_data(nc_tensor *t, int write);
 /* nc_backward from any f32 tensor y with dy as the gradient of it (same shape, any strides, same context)
- * instead of a scalar loss with gradient 1. dy is read, never written or kept. Returns the context status. */
+ * instead of a scalar loss with gradient 1. dy is read, never written or kept; it may be a gradient that a pass
+ * left (a retained one's of an intermediate tensor keeps its values until nc_step_end; a leaf's is read as it was
+ * and then added to, as in every pass). Returns the context status. */
 NC_API int nc_ext_backward_from(nc_tensor *y, nc_tensor *dy);
 
 /* ---- query/key norms with rotary positions -------------------------------------------------------

@@ -273,28 +273,37 @@ static void plan_release_node(nc_ctx *ctx, nc_node *n, nc_tensor *loss, const bw
 
 nc_status nc_backward(nc_tensor *loss) { return nc_backward_ex(loss, 0, NULL, 0); }
 
-/* whether dy's memory is (part of) a gradient that the pass may write */
-static int plan_writes(const bw_plan *pl, const nc_tensor *dy) {
-    const nc_tensor *o = nc__owner((nc_tensor *)dy);
-    const char *a = (const char *)o->data, *b = a + o->bytes;
+/* whether two pieces of device memory share a byte */
+static int overlap(const nc_tensor *g, const char *a, size_t bytes) {
+    const char *c = (const char *)g->data;
+    return c < a + bytes && a < c + g->bytes;
+}
+
+/* Makes dy safe to read for the whole pass: its pending value is computed, and a gradient of an intermediate tensor
+ * that it is (part of), left by a retained pass, is taken off that tensor, which gets a new one, so dy stays as it is
+ * until the step ends. Returns 1 when dy is (part of) the gradient of a leaf, which the pass adds to. */
+static int hold_dy(const bw_plan *pl, nc_tensor *dy) {
+    nc__dev(dy);
+    const nc_tensor *o = nc__owner(dy);
+    const char *a = (const char *)o->data;
+    int leaf = 0;
     for (int k = 0; k < pl->order.n; k++) {
-        const nc_node *n = pl->order.v[k];
+        nc_node *n = pl->order.v[k];
+        if (n->out->grad && overlap(n->out->grad, a, o->bytes)) n->out->grad = NULL;
         for (int i = 0; i < n->n_in; i++) {
-            const nc_tensor *g = n->in[i]->grad;
-            if (!g) continue;
-            const char *c = (const char *)g->data;
-            if (c < b && a < c + g->bytes) return 1;
+            const nc_tensor *x = n->in[i];
+            if (!x->node && x->grad && overlap(x->grad, a, o->bytes)) leaf = 1;
         }
     }
-    return 0;
+    return leaf;
 }
 
 /* d loss / d loss at the start of a pass: 1, or dy (the gradient of y given by the caller). A y that some op
  * produced and that holds no gradient reads the context's constant 1, or the caller's buffer, in place (an alias
  * that owns nothing and is dropped when the pass ends: *lent = 1; a retained pass keeps the gradient 1, in a
- * buffer of its own), unless the pass adds to that buffer. Otherwise 1 or dy is stored into a fresh buffer or added to what is there. Returns 0 on
- * failure. */
-static int seed_gradient(nc_ctx *ctx, nc_tensor *y, nc_tensor *dy, const bw_plan *pl, int retain, int *lent) {
+ * buffer of its own), unless the pass adds to that buffer (written). Otherwise 1 or dy is stored into a fresh buffer
+ * or added to what is there. Returns 0 on failure. */
+static int seed_gradient(nc_ctx *ctx, nc_tensor *y, nc_tensor *dy, int written, int retain, int *lent) {
     *lent = 0;
     if (!dy && !retain && y->node && !y->grad) { /* the context's constant 1, the same for every pass */
         if (!ctx->one) {
@@ -308,8 +317,7 @@ static int seed_gradient(nc_ctx *ctx, nc_tensor *y, nc_tensor *dy, const bw_plan
         *lent = 1;
         return 1;
     }
-    if (dy && y->node && !y->grad && nc_is_contiguous(dy) && !plan_writes(pl, dy)) {
-        nc__dev(dy);
+    if (dy && y->node && !y->grad && nc_is_contiguous(dy) && !written) {
         y->grad = nc__tensor_alias(dy, 0);
         *lent = y->grad != NULL;
         return *lent;
@@ -385,6 +393,8 @@ static nc_status backward_pass(nc_tensor *loss, nc_tensor *dy, int flags, nc_ten
         return ctx->status;
     }
 
+    const int written = dy && hold_dy(&pl, dy); /* before the gradients that it may be are cleared */
+
     /* gradients of intermediate tensors start from zero in every pass */
     cudaStream_t s = (cudaStream_t)ctx->dev.stream;
     for (int k = 0; k < pl.order.n; k++) {
@@ -396,7 +406,7 @@ static nc_status backward_pass(nc_tensor *loss, nc_tensor *dy, int flags, nc_ten
     }
 
     int lent;
-    if (!seed_gradient(ctx, loss, dy, &pl, retain, &lent)) {
+    if (!seed_gradient(ctx, loss, dy, written, retain, &lent)) {
         plan_free(&pl);
         return ctx->status;
     }

@@ -1,0 +1,82 @@
+"""nc_ext_backward_from with a gradient that an earlier pass left: a retained pass keeps the gradients of intermediate
+tensors, and the pass that follows starts those from zero. The given gradient is read as it was and left as it was.
+
+Bounds: a sum of K products has at most K roundings of the sum of absolute values (3xTF32 drops 2^-21 of each product),
+and tanh and its slope 1 - y^2 are off by less than 2^-20 of 1.
+"""
+
+from __future__ import annotations
+
+import numpy as np
+import pytest
+
+from nchelp import Eng, capi, seeded
+
+pytestmark = pytest.mark.gpu
+E = 2.0 ** -24
+RETAIN = 2
+N = 24  # square, so that every gradient of the graph can stand for every other one
+
+
+def build(e):
+    """x and w (leaves), h = x w^T, y = tanh(h) and z = y w^T, after a retained pass from sum(z * G)"""
+    tx, tw = e.param(seeded(1, (N, N))), e.param(seeded(2, (N, N), 0.3))
+    h = e.check(e.L.nc_linear_fn(tx, tw, None))
+    y = e.check(e.L.nc_tanh(h))
+    z = e.check(e.L.nc_linear_fn(y, tw, None))
+    loss = e.check(e.L.nc_sum(e.check(e.L.nc_mul(z, e.t(seeded(3, (N, N))))), capi.ALL_AXES, 0))
+    assert e.L.nc_backward_ex(loss, RETAIN, None, 0) == 0, e.err()
+    for t in (tx, tw):
+        e.L.nc_clear_grad(t)
+    return tx, tw, dict(h=h, y=y, z=z)
+
+
+def formula(root, dy):
+    """gradients of x and w from d root = dy, and the sums of absolute values that their bounds multiply"""
+    x, w, dy = seeded(1, (N, N)).astype(np.float64), seeded(2, (N, N), 0.3).astype(np.float64), dy.astype(np.float64)
+    y = np.tanh(x @ w.T)
+    gw, gws, size = np.zeros((N, N)), np.zeros((N, N)), abs(dy)
+    if root == "z":
+        gw, gws = dy.T @ y, size.T @ abs(y)
+        dy, size = dy @ w, size @ abs(w)
+    if root in ("z", "y"):
+        dy = dy * (1 - y * y)
+    return dy @ w, size @ abs(w), gw + dy.T @ x, gws + size.T @ abs(x)
+
+
+@pytest.mark.parametrize("kind", ["whole", "view", "pending"])
+@pytest.mark.parametrize("root,of", [("y", "y"), ("h", "h"), ("y", "h"), ("z", "h"), ("z", "z"), ("z", "y")])
+def test_dy_is_a_gradient_that_a_retained_pass_left(root, of, kind):
+    with Eng("b200") as e:
+        tx, tw, t = build(e)
+        g = e.check(e.L.nc_grad(t[of]))
+        left = e.np(g)
+        assert left.any()
+        dy, value = g, left
+        if kind == "view":
+            dy, value = e.check(e.L.nc_transpose(g, 0, 1)), left.T
+        elif kind == "pending":
+            dy, value = e.check(e.L.nc_gelu(g, 0)), e.np(e.check(e.L.nc_gelu(e.t(left), 0)))
+        assert e.L.nc_ext_backward_from(t[root], dy) == 0, e.err()
+        gx, gxs, gw, gws = formula(root, value)
+        unit = 3 * N * E + 2.0 ** -18
+        assert np.all(abs(e.grad(tx) - gx) <= unit * gxs) and np.all(abs(e.grad(tw) - gw) <= unit * gws)
+        assert np.array_equal(e.np(dy), value)  # as it was
+        if kind != "pending":
+            assert np.array_equal(e.np(g), left)
+        assert e.ok(), e.err()
+
+
+def test_two_passes_from_the_same_left_gradient():
+    with Eng("b200") as e:
+        tx, tw, t = build(e)
+        g = e.check(e.L.nc_grad(t["y"]))
+        left = e.np(g)
+        grads = []
+        for _ in range(2):
+            assert e.L.nc_ext_backward_from(t["z"], g) == 0, e.err()
+            grads.append((e.grad(tx), e.grad(tw)))
+            for p in (tx, tw):
+                e.L.nc_clear_grad(p)
+        assert all(np.array_equal(a, b) for a, b in zip(*grads)) and grads[0][0].any()
+        assert np.array_equal(e.np(g), left)
