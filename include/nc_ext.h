@@ -184,7 +184,9 @@ NC_API nc_optim *nc_ext_adamw8(nc_ctx *ctx, nc_tensor **params, int n, nc_optim_
 /* The moments of an optimizer that keeps two (Adam, AdamW, AdamW in 8 bits, RMSprop with momentum: its momentum
  * and square average) copied to or from a contiguous f32 tensor [2, elements] on the device: row 0 m, row 1 v, the parameters one
  * after the other. 8-bit moments are decoded and encoded; encoding what was decoded restores them bit for
- * bit. Together with nc_optim_get_step / set_step a checkpoint without a host copy. Return the context status. */
+ * bit. Together with nc_optim_get_step / set_step a checkpoint without a host copy. get_state
+ * shows what was written through nc_optim_state's pointers, and they stay good for more until the next step;
+ * put_state replaces everything and ends them (take them again). Return the context status. */
 NC_API int nc_ext_optim_get_state(nc_optim *o, nc_tensor *values);
 NC_API int nc_ext_optim_put_state(nc_optim *o, nc_tensor *values);
 

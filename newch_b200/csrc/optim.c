@@ -511,8 +511,10 @@ static int move_state(nc_optim *o, nc_tensor *t, int put) {
     if (!o || !t) return NC_ERR_ARG;
     nc_ctx *ctx = o->ctx;
     if (ctx->status != NC_OK || !state_tensor_ok(o, t, put ? "optim_put_state" : "optim_get_state")) return ctx->status;
-    state_upload_if_dirty(o);
     if (!put) {
+        const int shown = o->state_host_dirty; /* nc_optim_state's pointer is out: more may be written through it */
+        state_upload_if_dirty(o);
+        o->state_host_dirty = shown; /* the step takes the mirror again (the same floats give the same codes) */
         nc__deferred_flush(ctx); /* pending recipes may read the tensor */
         nc__dev_write(t);
     }
@@ -532,7 +534,7 @@ static int move_state(nc_optim *o, nc_tensor *t, int put) {
             at += n;
         }
     }
-    if (put) o->state_host_valid = 0;
+    if (put) o->state_host_valid = o->state_host_dirty = 0; /* all of it is replaced */
     return ctx->status;
 }
 
