@@ -141,7 +141,8 @@ NC_API nc_tensor *nc_ext_qk_norm_rope(nc_tensor *x, nc_tensor *q_weight, nc_tens
  * the logits. Rows that the mask leaves out are not read: their logits, labels and other entries may hold
  * anything, and their gradient is 0. A counted label outside [0, vocab) is an error (found on the device at
  * the latest: NC_ERR_ARG at the next synchronisation). Logits of -infinity have probability 0. Log
- * probabilities are summed and compared in 64 bits; sums run in the same order every time.
+ * probabilities are subtracted and summed, and the KL term formed, in 64 bits, ratios and what is clipped of them
+ * in 32; sums run in the same order every time.
  *
  * Everything but the logits is a constant: while gradients are enabled, an input of the others that requires
  * grad is refused. */

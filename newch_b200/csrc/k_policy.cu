@@ -17,8 +17,8 @@
 // a warp's lanes, so that the double precision arithmetic of the loss runs once for all of them and not once a row.
 // Backward deals rows out as blocks end (uncounted rows cost a third, so dealing them out in advance leaves SMs idle:
 // with a mask 418 instead of 352 us) and starts with the last long row, whose logits the forward pass may have left in
-// L2. Log probabilities and everything behind them that can cancel (log ratios, sums over tokens and rows) are held in
-// 64 bits; sums run in a fixed order.
+// L2. Log probabilities and everything behind them that can cancel (log ratios, the KL term, sums over tokens and rows)
+// are held in 64 bits, a row's ratio and its product with the advantage in 32; sums run in a fixed order.
 #include <math.h>
 
 #include "k_common.cuh"
@@ -258,6 +258,13 @@ __device__ __forceinline__ RowIn row_in(const nck_rows &q, const nck_policy &p, 
     return in;
 }
 
+// e^a - 1 - a from e = e^a - 1, never negative: the two cancel near 0 (a policy near its reference), where the series'
+// next term is below 2^-29 of the sum, and both are infinite for an action of probability 0.
+__device__ __forceinline__ double exp_rest(double a, double e) {
+    if (fabs(a) < 1.220703125e-4) return a * a * (0.5 + a * (1.0 / 6.0)); // 2^-13
+    return isinf(e) ? e : e - a;
+}
+
 // What a row's log probability becomes: its loss term and the factor c of its gradient (without 1 / count).
 __device__ __forceinline__ double policy_term(const nck_policy &p, const RowIn &in, double lp, float *c) {
     const float A = in.adv, ratio = expf((float)(lp - (double)in.old));
@@ -265,14 +272,15 @@ __device__ __forceinline__ double policy_term(const nck_policy &p, const RowIn &
     const float held = fminf(fmaxf(ratio, lo), hi);
     const float gain = fminf(ratio * A, held * A);
     const bool moves = A >= 0.0f ? ratio <= hi : ratio >= lo, lost = isnan(ratio) || isnan(A);
-    float term = lost ? ratio + A : -gain, f = lost ? ratio + A : moves ? -A * ratio : 0.0f;
+    double term = lost ? ratio + A : -gain;
+    float f = lost ? ratio + A : moves ? -A * ratio : 0.0f;
     if (p.kl != 0.0f) {
-        const float away = (float)((double)in.ref - lp), e = expm1f(away);
-        term += p.kl * (e - away);
-        f -= p.kl * e;
+        const double away = (double)in.ref - lp, e = expm1(away);
+        term += (double)p.kl * exp_rest(away, e);
+        f -= p.kl * (float)e;
     }
     *c = f;
-    return (double)term;
+    return term;
 }
 
 __device__ __forceinline__ Sums finish_row(const nck_rows &q, const nck_policy &p, int64_t r, Stat st, const RowIn &in) {
