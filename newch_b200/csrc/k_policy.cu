@@ -519,7 +519,9 @@ __global__ void __launch_bounds__(256) k_pairs(nck_pairs p, const double *lp, do
         }
         const double h = (double)p.beta * (seq[0] - seq[1]), eps = (double)p.smoothing;
         const double soft = log1p(exp(-fabs(h)));  // softplus(-|h|)
-        term[i] = (1.0 - eps) * (soft + (h < 0.0 ? -h : 0.0)) + eps * (soft + (h > 0.0 ? h : 0.0));
+        double loss = (1.0 - eps) * (soft + (h < 0.0 ? -h : 0.0));
+        if (eps > 0.0) loss += eps * (soft + (h > 0.0 ? h : 0.0)); // (an infinite h times a weight of 0 is NaN)
+        term[i] = loss;
         if (p.coef) {
             const double c = (double)p.beta / (double)p.P * (1.0 / (1.0 + exp(-h)) - (1.0 - eps));
             p.coef[i] = (float)c;

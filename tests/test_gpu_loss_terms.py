@@ -86,3 +86,32 @@ def test_kl_term_of_an_impossible_action_is_infinite(V):
         assert loss == np.inf and np.isfinite(g).all()
         loss, g = policy(e, z, act, np.full(2, -1, F), None, np.ones(2, F), 0.0)  # without a KL term: a ratio of 0
         assert np.isfinite(loss) and np.isfinite(g).all() and not g[0].any()
+
+
+@pytest.mark.parametrize("V", [4, 700, 20000])
+def test_preference_of_an_impossible_answer(V):
+    """An answer with a token of probability 0: h is infinite, and without smoothing the pair's loss is 0 where the
+    impossible answer is the other one (log sigmoid(-h) has weight 0) and infinite where it is the preferred one."""
+    T = 3
+    for side in (0, 1):
+        z = np.random.default_rng(V).standard_normal((4, T, V)).astype(F)
+        lab = np.zeros((4, T), np.int32)
+        z[2 * side, 1, 0] = -np.inf  # a token of the first pair's preferred answer, or of its other one
+        with Eng("b200") as e:
+            def run(eps):
+                tz = e.param(z)
+                loss = e.check(e.L.nc_ext_preference_loss(tz, e.t(lab), None, None, 0.5, eps, None))
+                assert e.L.nc_backward(loss) == 0, e.err()
+                return float(e.np(loss)), e.grad(tz)
+
+            loss, g = run(0.0)
+            lp = z.astype(np.float64) - np.log(np.exp(z.astype(np.float64)).sum(-1, keepdims=True))
+            h = 0.5 * (lp[1, :, 0].sum() - lp[3, :, 0].sum())  # the second pair
+            if side:
+                # lp is off by (8 max|z| + 64 + V / 32) e as everywhere, and T of them make a sum
+                unit = (8 * 6 + 64 + V / 32) * E
+                assert abs(loss - np.log1p(np.exp(-h)) / 2) <= 2 * T * unit * 0.5 + 4 * E
+                assert np.isfinite(g).all() and not g[0].any() and not g[2].any() and g[1].any()
+            else:
+                assert loss == np.inf and np.isfinite(g[1]).all() and np.isfinite(g[3]).all()
+            assert run(0.1)[0] == np.inf
