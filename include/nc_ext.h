@@ -177,8 +177,9 @@ NC_API nc_tensor *nc_ext_preference_loss(nc_tensor *logits, nc_tensor *labels, n
  * moments are kept as one byte an element and an fp32 maximum s per block of 256 elements of a parameter,
  *   m = sign(c) s (c / 127)^2, c in [-127, 127];   v = s (c / 255)^4, c in [0, 255], 0 for v = 0 only,
  * each rounded to the nearest code (in sqrt|m| and v^(1/4)) after the step. The step uses the moments before
- * that rounding, in fp32. Blocks whose largest value is below 2^-94 count as zero; a gradient that is not
- * finite makes the moments of its block not finite. The handle works with every nc_optim_* call, gradient
+ * that rounding, in fp32. Blocks whose largest value is below 2^-94 count as zero; a v beyond fp32, from
+ * a finite gradient, is held as the largest float (the step itself divides by infinity: it moves nothing); a gradient
+ * that is not finite makes the moments of its block not finite. The handle works with every nc_optim_* call, gradient
  * accumulation and data parallelism included; nc_optim_state shows the moments as floats, and floats written
  * through it are encoded again before the next step (v by its absolute value). Defaults as nc_adamw. */
 NC_API nc_optim *nc_ext_adamw8(nc_ctx *ctx, nc_tensor **params, int n, nc_optim_opts opts);

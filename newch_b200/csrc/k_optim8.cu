@@ -97,12 +97,22 @@ __device__ __forceinline__ float warp_largest(float top) {
     return s < kLeast ? 0.0f : s;
 }
 
-// The lane's eight elements' moments (0 past the end) to codes, and the block's largest values.
-__device__ __forceinline__ uint4 encode(const float (&m)[8], const float (&v)[8], float2 &top) {
-    float a = fabsf(m[0]), b = v[0];
+__device__ __forceinline__ float largest_of(const float (&v)[8]) {
+    float a = fabsf(v[0]);
 #pragma unroll
-    for (int i = 1; i < 8; i++) a = larger(a, fabsf(m[i])), b = larger(b, v[i]);
-    top = make_float2(warp_largest(a), warp_largest(b));
+    for (int i = 1; i < 8; i++) a = larger(a, fabsf(v[i]));
+    return warp_largest(a);
+}
+
+// The lane's eight elements' moments (0 past the end) to codes, and the block's largest values. `hold` is called, by
+// all lanes, when the largest v is infinite, and may change v.
+template <typename F>
+__device__ __forceinline__ uint4 encode(const float (&m)[8], float (&v)[8], float2 &top, F hold) {
+    top = make_float2(largest_of(m), largest_of(v));
+    if (top.y == INFINITY) {
+        hold();
+        top.y = largest_of(v);
+    }
     const float rm = top.x > 0.0f ? (1.0f / top.x) * kFullM : 0.0f, rv = top.y > 0.0f ? (1.0f / top.y) * kFullV : 0.0f;
     const float least = top.y > 0.0f ? 1.0f : 0.0f;
     uint32_t w[4];
@@ -175,7 +185,19 @@ __global__ void __launch_bounds__(256) k_adamw8(Step8 h, nck_opt8 q, const nck_o
     }
 #pragma unroll
     for (int k = 0; k < 2; k++) put4(w, n, k * 128 + lane * 4, wv + 4 * k);
-    *codes = encode(m, v, top);
+    // A finite gradient whose square is not (above about 6e20) would make its block's largest v infinite and the other
+    // 255 elements' v with it: it is held as the largest float. (Asked of the largest alone: a test of every element
+    // took 9 registers more.)
+    const bool was_finite = top.y < INFINITY;
+    *codes = encode(m, v, top, [&]() {
+        if (!was_finite) return;
+        float gj[8];
+#pragma unroll
+        for (int k = 0; k < 2; k++) get4(g, n, k * 128 + lane * 4, gj + 4 * k);
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+            if (v[i] == INFINITY && fabsf(gj[i]) < INFINITY) v[i] = 3.402823466e38f;
+    });
     if (lane == 0) *tops = top;
 }
 
@@ -237,7 +259,7 @@ __global__ void __launch_bounds__(256) k_opt8_values(nck_opt8 q, const nck_opt8_
             v[i] = at < n ? fabsf(vs[at]) : 0.0f;
         }
         float2 top;
-        reinterpret_cast<uint4 *>(codes)[lane] = encode(m, v, top);
+        reinterpret_cast<uint4 *>(codes)[lane] = encode(m, v, top, []() {});
         if (lane == 0) *tops = top;
     } else {
         const float2 top = *tops;

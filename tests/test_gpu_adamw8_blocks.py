@@ -1,0 +1,49 @@
+"""nc_ext_adamw8: what one element of a block of 256 does to the others, and which lists of parameters it takes."""
+
+from __future__ import annotations
+
+import numpy as np
+import pytest
+
+from nchelp import Eng, capi
+from test_gpu_adamw8 import BLOCK, F, Emulated, give, opts, optimizer, same_bits, state, through_codes
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("big", [7e20, -1e21, 3e38])
+def test_a_finite_gradient_leaves_its_block_finite(big):
+    """The square of a gradient above about 6e20 is beyond fp32: v is held as the largest finite float, so that the
+    other 255 elements keep finite moments and weights. A gradient of infinity still makes its block not finite."""
+    rng = np.random.default_rng(1)
+    n = 3 * BLOCK + 40
+    w = rng.standard_normal(n).astype(F)
+    top = np.finfo(F).max
+    m, v = np.zeros(n, F), np.zeros(n, F)
+    with Eng("b200") as e:
+        t = e.param(w)
+        o = optimizer(e, [t], opts(decay=0.0))
+        for k in range(4):
+            g = rng.standard_normal(n).astype(F)
+            g[BLOCK:BLOCK + 8] = 0
+            g[BLOCK + 9] = big
+            if k == 0:
+                g[-1] = np.inf
+            before = e.np(t)
+            give(e, [t], [g])
+            e.L.nc_optim_step(o)
+            got = state(e, o, n)
+            with np.errstate(all="ignore"):
+                m = F(0.9) * m + (F(1) - F(0.9)) * g
+                v = F(0.999) * v + ((F(1) - F(0.999)) * g) * g
+            v = np.where(np.isinf(v) & np.isfinite(g), top, v)
+            m, v = through_codes(m, v)
+            ok = slice(0, 3 * BLOCK)
+            assert np.isfinite(got[:, ok]).all(), k
+            assert same_bits(got[0][ok], m[ok]) and same_bits(got[1][ok], v[ok]), k
+            assert got[1][BLOCK + 9] == top
+            assert np.isfinite(e.np(t)[ok]).all()
+            assert not np.isfinite(got[0][3 * BLOCK:]).any() and not np.isfinite(got[1][3 * BLOCK:]).any()
+            if k == 0:  # the step divides by the moment before it is held: an infinite one moves nothing
+                assert e.np(t)[BLOCK + 9] == before[BLOCK + 9]
+        e.L.nc_optim_free(o)
