@@ -181,7 +181,7 @@ NC_API nc_tensor *nc_ext_preference_loss(nc_tensor *logits, nc_tensor *labels, n
  * a finite gradient, is held as the largest float (the step itself divides by infinity: it moves nothing); a gradient
  * that is not finite makes the moments of its block not finite. The handle works with every nc_optim_* call, gradient
  * accumulation and data parallelism included; nc_optim_state shows the moments as floats, and floats written
- * through it are encoded again before the next step (v by its absolute value). Defaults as nc_adamw. */
+ * through it are encoded again before the next step (v by its absolute value). Defaults as nc_adamw. A parameter is given once. */
 NC_API nc_optim *nc_ext_adamw8(nc_ctx *ctx, nc_tensor **params, int n, nc_optim_opts opts);
 /* The moments of an optimizer that keeps two (Adam, AdamW, AdamW in 8 bits, RMSprop with momentum: its momentum
  * and square average) copied to or from a contiguous f32 tensor [2, elements] on the device: row 0 m, row 1 v, the parameters one

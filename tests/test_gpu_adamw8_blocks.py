@@ -47,3 +47,18 @@ def test_a_finite_gradient_leaves_its_block_finite(big):
             if k == 0:  # the step divides by the moment before it is held: an infinite one moves nothing
                 assert e.np(t)[BLOCK + 9] == before[BLOCK + 9]
         e.L.nc_optim_free(o)
+
+
+def test_a_parameter_is_taken_once():
+    """The same parameter twice would be stepped by two blocks at once: refused, and nothing is changed."""
+    with Eng("b200") as e:
+        a, b = e.param(np.ones(300, F)), e.param(np.ones(5, F))
+        give(e, [a, b], [np.full(300, 2, F), np.full(5, 3, F)])
+        for ts in ([a, a], [a, b, a]):
+            assert not e.L.nc_ext_adamw8(e.ctx, capi.ptr_array(ts), len(ts), opts()) and "twice" in e.err()
+            e.L.nc_clear_error(e.ctx)
+        assert np.array_equal(e.grad(a), np.full(300, 2, F)) and np.array_equal(e.grad(b), np.full(5, 3, F))
+        o = optimizer(e, [a, b])
+        e.L.nc_optim_step(o)
+        assert e.ok() and (e.np(a) < 1).all() and (e.np(b) < 1).all()
+        e.L.nc_optim_free(o)
