@@ -337,12 +337,17 @@ nc_optim *nc_ext_adamw8(nc_ctx *ctx, nc_tensor **params, int n, nc_optim_opts op
         nc__error(ctx, NC_ERR_ARG, "adamw8: no parameters given");
         return NULL;
     }
-    for (int i = 1; i < n; i++)
+    for (int i = 0; i < n; i++) {
+        if (params[i] && params[i]->ctx != ctx) { /* its work is ordered by another stream */
+            nc__error(ctx, NC_ERR_ARG, "adamw8: param %d belongs to another context", i);
+            return NULL;
+        }
         for (int j = 0; j < i; j++)
             if (params[i] && params[i] == params[j]) { /* two blocks would step the same weights at once */
                 nc__error(ctx, NC_ERR_ARG, "adamw8: params %d and %d are the same parameter, given twice", j, i);
                 return NULL;
             }
+    }
     return create(ctx, OPT_ADAMW8, params, n, adam_defaults(opts));
 }
 

@@ -62,3 +62,15 @@ def test_a_parameter_is_taken_once():
         e.L.nc_optim_step(o)
         assert e.ok() and (e.np(a) < 1).all() and (e.np(b) < 1).all()
         e.L.nc_optim_free(o)
+
+
+def test_a_parameter_of_another_context_is_refused():
+    with Eng("b200") as e, Eng("b200") as other:
+        a, b = e.param(np.ones(300, F)), other.param(np.ones(300, F))
+        assert not e.L.nc_ext_adamw8(e.ctx, capi.ptr_array([a, b]), 2, opts()) and "another context" in e.err()
+        e.L.nc_clear_error(e.ctx)
+        give(other, [b], [np.full(300, 2, F)])
+        o = optimizer(other, [b])
+        other.L.nc_optim_step(o)
+        assert e.ok() and other.ok() and (other.np(b) < 1).all() and e.grad(a) is None
+        other.L.nc_optim_free(o)
