@@ -359,6 +359,10 @@ int nc_ext_backward_from(nc_tensor *y, nc_tensor *dy) {
         nc__error(ctx, NC_ERR_ARG, "backward_from: inputs belong to different contexts");
         return ctx->status;
     }
+    if (nc__is_released(dy)) {
+        nc__error(ctx, NC_ERR_STATE, "backward_from: the gradient was released");
+        return ctx->status;
+    }
     if (y->dtype != NC_F32 || dy->dtype != NC_F32) {
         nc__error(ctx, NC_ERR_DTYPE, "backward_from: the tensor and its gradient must be f32");
         return ctx->status;

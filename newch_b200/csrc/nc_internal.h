@@ -302,6 +302,8 @@ int nc__expect_f32(const nc_node *n, int i);
 nc_tensor *nc__tensor_new(nc_ctx *ctx, nc_dtype dt, int ndim, const int64_t *shape, int persistent);
 nc_tensor *nc__tensor_alias(const nc_tensor *src, int persistent);
 static inline nc_tensor *nc__owner(nc_tensor *t) { return t->owner ? t->owner : t; }
+/* whether t's memory was given back (nc_release_temp, or a backward pass that frees its graph); a view's is its owner's */
+static inline int nc__is_released(const nc_tensor *t) { return !t->data || !nc__owner((nc_tensor *)t)->data; }
 
 nc_tensor *nc__grad_buf(nc_tensor *t);
 /* The gradient buffer for a writer that sets every element of it: a new (or zero_grad-cleared)

@@ -31,6 +31,10 @@ static int refuse(nc_ctx *ctx, nc_status code, const char *op, const char *what)
 static int inputs_ok(const char *op, nc_tensor *z, nc_tensor *const given[5]) {
     static const char *const names[5] = {"labels", "old_logp", "ref_logp", "advantages", "mask"};
     nc_ctx *ctx = z->ctx;
+    for (int i = -1; i < 5; i++) {
+        const nc_tensor *t = i < 0 ? z : given[i];
+        if (t && nc__is_released(t)) return refuse(ctx, NC_ERR_STATE, op, "an input was released");
+    }
     if (z->dtype != NC_F32) return refuse(ctx, NC_ERR_DTYPE, op, "logits must be f32");
     if ((z->ndim != 2 && z->ndim != 3) || z->shape[z->ndim - 1] < 1 || z->shape[z->ndim - 1] > INT32_MAX)
         return refuse(ctx, NC_ERR_SHAPE, op, "logits must be [rows, vocab] or [batch, tokens, vocab], 1 <= vocab < 2^31");
@@ -176,9 +180,9 @@ static void policy_bwd(nc_node *n) { loss_bwd(n, 1, 1); }
 
 const nc_op_def nc_op_policy_loss = {"policy_loss", 0, 0, loss_infer, NULL, policy_fwd, policy_bwd};
 
-/* a mask of another integer type becomes i32, as masked_fill's does */
+/* a mask of another integer type becomes i32, as masked_fill's does (a released one is refused with the rest) */
 static nc_tensor *as_mask(nc_tensor *mask) {
-    return mask && (mask->dtype == NC_I8 || mask->dtype == NC_U8) ? nc_to_dtype(mask, NC_I32) : mask;
+    return mask && !nc__is_released(mask) && (mask->dtype == NC_I8 || mask->dtype == NC_U8) ? nc_to_dtype(mask, NC_I32) : mask;
 }
 
 nc_tensor *nc_ext_policy_loss(nc_tensor *logits, nc_tensor *actions, nc_tensor *old_logp, nc_tensor *ref_logp,

@@ -24,6 +24,8 @@ static nc_status refuse(nc_ctx *ctx, nc_status code, const char *what) {
 static nc_status rope_infer(nc_node *n, nc_dtype *dt, int *nd, int64_t *shape) {
     nc_tensor *x = n->in[0];
     nc_ctx *ctx = x->ctx;
+    for (int i = 0; i < n->n_in; i++)
+        if (nc__is_released(n->in[i])) return refuse(ctx, NC_ERR_STATE, "an input was released");
     if (!nc__expect_f32(n, 0)) return NC_ERR_DTYPE;
     if (x->ndim != 4) return refuse(ctx, NC_ERR_SHAPE, "x must be [batch, tokens, heads, dim]");
     const int64_t H = x->shape[2], D = x->shape[3], A = n->p.i[P_AXES];

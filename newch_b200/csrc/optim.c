@@ -505,6 +505,10 @@ static int state_tensor_ok(nc_optim *o, const nc_tensor *t, const char *what) {
         nc__error(ctx, NC_ERR_ARG, "%s: the tensor belongs to another context", what);
         return 0;
     }
+    if (nc__is_released(t)) {
+        nc__error(ctx, NC_ERR_STATE, "%s: the tensor was released", what);
+        return 0;
+    }
     if (t->dtype != NC_F32) {
         nc__error(ctx, NC_ERR_DTYPE, "%s: the tensor must be f32", what);
         return 0;

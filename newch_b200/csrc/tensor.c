@@ -566,7 +566,7 @@ nc_tensor *nc__grad_buf_set(nc_tensor *t, int *acc) {
 }
 
 void *nc_ext_device_data(nc_tensor *t, int write) {
-    if (!t || !t->data || t->ctx->status != NC_OK) return NULL;
+    if (!t || nc__is_released(t) || t->ctx->status != NC_OK) return NULL;
     void *p = nc__dev(t);
     if (write) {
         nc__deferred_flush(t->ctx); /* pending recipes may read what the caller is about to change */
