@@ -80,3 +80,36 @@ def test_two_passes_from_the_same_left_gradient():
                 e.L.nc_clear_grad(p)
         assert all(np.array_equal(a, b) for a, b in zip(*grads)) and grads[0][0].any()
         assert np.array_equal(e.np(g), left)
+
+
+@pytest.mark.parametrize("first", [0, 1, 2, 3])
+@pytest.mark.parametrize("op", ["tanh", "linear", "layer_norm", "softmax", "rope"])
+def test_dy_begins_at_any_element(op, first):
+    """A contiguous dy within a larger tensor, off every 16-byte boundary, is read where it is: the gradients are those
+    of a dy with memory of its own, but for the order of sums."""
+    import ctypes
+
+    B, D = 64, 128
+    x, w, dy = seeded(1, (B, D)), seeded(2, (D, D), 0.2), seeded(3, (B, D))
+    with Eng("b200") as e:
+        tx, tw, tv = e.param(x), e.param(w), e.param(1 + w[0])
+        o = capi.RopeOpts(1, 1, (ctypes.c_int * 3)(16), 10000.0, 1e-6, 0)
+        run = {"tanh": lambda: e.L.nc_tanh(tx), "linear": lambda: e.L.nc_linear_fn(tx, tw, tv),
+               "layer_norm": lambda: e.L.nc_layer_norm(tx, 1, tv, None, 1e-5), "softmax": lambda: e.L.nc_softmax(tx),
+               "rope": lambda: e.L.nc_reshape(e.check(e.L.nc_ext_qk_norm_rope(
+                   e.check(e.L.nc_reshape(tx, *capi.shape_arg((1, B, 4, 32)))), None, None, None, ctypes.byref(o))),
+                   *capi.shape_arg((B, D)))}[op]
+        got = []
+        for at in (None, first):
+            flat = e.t(np.concatenate((np.zeros(at or 0, np.float32), dy.ravel())))
+            td = flat if at is None else e.check(e.L.nc_slice(flat, 0, at, B * D, 1))
+            td = e.check(e.L.nc_reshape(td, *capi.shape_arg((B, D))))
+            assert e.L.nc_ext_backward_from(e.check(run()), td) == 0, e.err()
+            got.append([e.grad(t) for t in (tx, tw, tv)])
+            for t in (tx, tw, tv):
+                e.L.nc_clear_grad(t)
+            assert np.array_equal(e.np(td), dy)
+        for a, b in zip(*got):
+            assert (a is None) == (b is None)
+            assert a is None or np.abs(a - b).max() <= 2 * B * E * np.abs(a).max() + 1e-30
+        assert got[0][0].any() and e.ok(), e.err()
