@@ -16,9 +16,11 @@
 // of 72: 88 instead of 102 us; 4 x 8000 x 16 heads of 66 69 instead of 131).
 //
 // Angles are formed in whole numbers: a pair's turns per step are kept as a 64-bit fraction of a turn, a
-// position times it modulo 2^64 is the fraction of the turn reached, exact to 2^-34 turns at any i32 position,
-// and its upper half splits into quarter turns and a remainder of at most 1/8 turn. On that range sine and cosine
-// are polynomials (interpolation in the remainder's square at Chebyshev nodes), off by less than 1.6 * 2^-24.
+// position times it modulo 2^64 is the fraction of the turn reached, and its upper half (cut off below 2^-32 turns)
+// splits into quarter turns and a remainder of at most 1/8 turn. The steps are off by 9 units of 2^-64 at most for
+// bases above 1 (3 for 10000; ops_rope.c), so the angle is by 2^-32 + |position| 9 * 2^-64 turns: below 2^-29 at any i32
+// position, a fifth of 2^-24 in radians. On that range sine and cosine are polynomials (interpolation in the remainder's
+// square at Chebyshev nodes), off by less than 1.9 * 2^-24 with the rounding of the remainder.
 #include "k_common.cuh"
 
 using namespace nck;

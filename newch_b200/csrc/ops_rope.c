@@ -89,9 +89,12 @@ static int rope_of(const nc_node *n, nck_rope *q) {
     q->pos_b = pos && pos->ndim == 3 ? q->T * q->n_axes : 0;
     if (!q->x || (wq && !q->wq) || (wk && !q->wk) || (pos && !q->pos)) return 0;
     /* Turns of pair i per step, base^-(i / half) / 2 pi, as fractions of 2^64: the first one times the ratio of
-     * neighbours again and again, in 64 by 64 bits (off by less than 2^-59 turns after 127 products, as each adds
-     * half a unit and the ratio shrinks what is there), or in long double for a base below 1, whose turns
-     * grow past whole ones. With AXIS_FREQ i counts from the start of its section and half is the section's length. */
+     * neighbours again and again, in 64 by 64 bits. A product adds half a unit, and the ratio's own error (a unit or
+     * two of 2^-64) at most a sixth of it for each, so 128 pairs are off by less than 2^-57 at worst; replayed against
+     * 60 digits for bases from 1.0000001 to 1e30 and 1 to 128 pairs it is 9 units of 2^-64 at most, 3 for a base of
+     * 10000. In long double for a base of 1 or less, whose turns grow past whole ones: off by 2^-58 for a base of 0.5
+     * (128 pairs), and in proportion to the largest turn below that. With AXIS_FREQ i counts from the start of its
+     * section and half is the section's length. */
     const long double unit = 0.159154943091895335768883763372514362L, two64 = 0x1p64L, ln_base = logl((long double)n->p.f[0]);
     const int half = q->D / 2, by_axis = (n->p.i[P_FLAGS] & NC_EXT_ROPE_AXIS_FREQ) != 0;
     const uint64_t first = (uint64_t)(unit * two64);
