@@ -510,6 +510,7 @@ nc_tensor *nc__grad_buf(nc_tensor *t) {
         ctx->grad_alloc = 1;
         t->grad = nc__tensor_new(ctx, NC_F32, t->ndim, t->shape, persistent);
         ctx->grad_alloc = 0;
+        t->flags &= ~NC_TF_GRAD_CLEARED; /* (of a gradient that is gone) */
         if (t->grad)
             nc__cuda_ok(ctx, cudaMemsetAsync(t->grad->data, 0, t->grad->bytes, (cudaStream_t)ctx->dev.stream),
                         "memset");
@@ -548,6 +549,7 @@ nc_tensor *nc__grad_buf_acc(nc_tensor *t, int *acc) {
     ctx->grad_alloc = 1;
     t->grad = nc__tensor_new(ctx, NC_F32, t->ndim, t->shape, 0);
     ctx->grad_alloc = 0;
+    t->flags &= ~NC_TF_GRAD_CLEARED; /* (of a gradient that is gone) */
     if (t->grad) *acc = 0;
     return t->grad;
 }
@@ -561,6 +563,7 @@ nc_tensor *nc__grad_buf_set(nc_tensor *t, int *acc) {
     }
     if (t->grad || !(t->flags & NC_TF_PERSISTENT)) return nc__grad_buf_acc(t, acc);
     t->grad = nc__tensor_new(t->ctx, NC_F32, t->ndim, t->shape, 1);
+    t->flags &= ~NC_TF_GRAD_CLEARED;
     *acc = 0;
     return t->grad;
 }

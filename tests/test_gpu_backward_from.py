@@ -113,3 +113,50 @@ def test_dy_begins_at_any_element(op, first):
             assert (a is None) == (b is None)
             assert a is None or np.abs(a - b).max() <= 2 * B * E * np.abs(a).max() + 1e-30
         assert got[0][0].any() and e.ok(), e.err()
+
+
+@pytest.mark.parametrize("cleared", [False, True])
+def test_a_left_gradient_of_a_tensor_with_two_consumers(cleared):
+    """h feeds two ops, so its new gradient is a sum of two; whether the old one, which is dy, was cleared before."""
+    with Eng("b200") as e:
+        tx, tw = e.param(seeded(1, (N, N))), e.param(seeded(2, (N, N), 0.3))
+        h = e.check(e.L.nc_linear_fn(tx, tw, None))
+        z = e.check(e.L.nc_mul(e.check(e.L.nc_tanh(h)), e.check(e.L.nc_sigmoid(h))))
+        loss = e.check(e.L.nc_sum(e.check(e.L.nc_mul(z, e.t(seeded(3, (N, N))))), capi.ALL_AXES, 0))
+        assert e.L.nc_backward_ex(loss, RETAIN, None, 0) == 0, e.err()
+        g = e.check(e.L.nc_grad(h))
+        left = e.np(g)
+        for t in (tx, tw) + ((h, z) if cleared else ()):
+            e.L.nc_clear_grad(t)
+        assert e.L.nc_ext_backward_from(z, g) == 0, e.err()
+        x, w = seeded(1, (N, N)).astype(np.float64), seeded(2, (N, N), 0.3).astype(np.float64)
+        y, s = np.tanh(x @ w.T), 1 / (1 + np.exp(-x @ w.T))
+        dh, size = left * ((1 - y * y) * s + y * s * (1 - s)), abs(left)
+        unit = 3 * N * E + 2.0 ** -18
+        assert np.all(abs(e.grad(tx) - dh @ w) <= unit * (size @ abs(w)))
+        assert np.all(abs(e.grad(tw) - dh.T @ x) <= unit * (size.T @ abs(x)))
+        assert np.array_equal(e.np(g), left)
+
+
+def test_a_cleared_gradient_that_a_pass_dropped():
+    """nc_backward's own way to the same place: a retained pass, the gradient of h cleared, a pass that does not reach
+    h's consumers but drops its gradient, and one that reaches both."""
+    with Eng("b200") as e:
+        tx = e.param(seeded(1, (N, N)))
+        h = e.check(e.L.nc_scale(tx, 0.5))
+        y, s = e.check(e.L.nc_tanh(h)), e.check(e.L.nc_sigmoid(h))
+        z = e.check(e.L.nc_mul(y, s))
+        loss = lambda t: e.check(e.L.nc_sum(t, capi.ALL_AXES, 0))  # noqa: E731
+        want = []
+        for clear in (False, True):
+            assert e.L.nc_backward_ex(loss(z), RETAIN, None, 0) == 0, e.err()
+            if clear:
+                e.L.nc_clear_grad(h)
+            assert e.L.nc_backward(loss(e.check(e.L.nc_scale(h, 2.0)))) == 0, e.err()
+            if clear:
+                e.L.nc_clear_grad(h)
+            e.L.nc_clear_grad(tx)
+            assert e.L.nc_backward(loss(z)) == 0, e.err()
+            want.append(e.grad(tx))
+            e.L.nc_clear_grad(tx)
+        assert np.array_equal(*want) and want[0].any()
